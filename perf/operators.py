@@ -320,8 +320,8 @@ def _plain_append(s):
         moved = _to_codes(was.view(cache.dtype).float() * ratio[:, :, None, None], cache.dtype).view(torch.uint8)
         raw[block] = torch.where(held[:, None, :, None], moved, was)
         scales[block] = new
-        mine = new[group][:, :, None]
-        fresh = _to_codes(torch.where(mine > 0, x / mine, 0.0), cache.dtype).view(torch.uint8)
+        steps = torch.where(new > 0, (1.0 / new).clamp(max=3.4028234e38), 0.0)  # steps of the code in 1
+        fresh = _to_codes(x * steps[group][:, :, None], cache.dtype).view(torch.uint8)
         raw[slots // bs, :, slots % bs] = fresh
     return dict(k_cache=s["k_cache"], v_cache=s["v_cache"], k_scale=s["k_scale"], v_scale=s["v_scale"])
 
