@@ -1,9 +1,10 @@
 """Build recipe for the package's native code, in-tree.
 
 Produces, next to this file:
-  libb2g_sm100.so           the C-ABI library (include/b2g_gemm.h): the
-                            tcgen05 GEMM engine, the row-scale kernel and the
-                            host dispatcher; nvcc, sm_100a only, no torch.
+  libb2g_sm100.so           the C-ABI library (include/b2g_gemm.h,
+                            include/b2g_serving.h): the tcgen05 GEMM engine,
+                            the row-scale kernel, the host dispatcher and the
+                            serving operators; nvcc, sm_100a only, no torch.
   _b2g_torch<ext-suffix>    the Torch C++ extension (forward(A, B) per
                             operator) linked against libb2g_sm100.so.
 
@@ -29,10 +30,11 @@ ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 LIB = PKG / "libb2g_sm100.so"
 EXT = PKG / ("_b2g_torch" + sysconfig.get_config_var("EXT_SUFFIX"))
 
-CU_SOURCES = [CSRC / "b2g_capi.cu", CSRC / "b2g_vector.cu", CSRC / "b2g_peer.cu"]
+CU_SOURCES = [CSRC / "b2g_capi.cu", CSRC / "b2g_vector.cu", CSRC / "b2g_peer.cu",
+              CSRC / "b2g_serving.cu", CSRC / "b2g_cache_attention.cu", CSRC / "b2g_prompt.cu"]
 CU_DEPS = CU_SOURCES + [CSRC / "gemm_engine.cuh", CSRC / "sdpa_engine.cuh", CSRC / "ptx_sm100.cuh",
-                        CSRC / "b2g_internal.h",
-                        INCLUDE / "b2g_gemm.h"]
+                        CSRC / "b2g_internal.h", CSRC / "peer_protocol.cuh",
+                        INCLUDE / "b2g_gemm.h", INCLUDE / "b2g_serving.h"]
 EXT_SOURCES = [CSRC / "torch_binding.cpp"]
 
 
@@ -51,7 +53,7 @@ def _run(cmd, verbose):
 
 def build_lib(verbose: bool = False, force: bool = False) -> Path:
     if force or _stale(LIB, CU_DEPS):
-        cmd = [NVCC, *ARCH, "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
+        cmd = [NVCC, *ARCH, "-t", "0", "-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC",
                "-Xcompiler", "-fvisibility=hidden", "-shared", "-I", INCLUDE,
                "-o", LIB, *CU_SOURCES]
         _run(cmd, verbose)
@@ -63,7 +65,7 @@ def build_ext(verbose: bool = False, force: bool = False) -> Path:
     from torch.utils import cpp_extension as ce
 
     build_lib(verbose, force)
-    if force or _stale(EXT, EXT_SOURCES + [LIB, INCLUDE / "b2g_gemm.h"]):
+    if force or _stale(EXT, EXT_SOURCES + [LIB, INCLUDE / "b2g_gemm.h", INCLUDE / "b2g_serving.h"]):
         incs = ce.include_paths() + [sysconfig.get_paths()["include"], str(CUDA_HOME / "include"),
                                      str(INCLUDE)]
         torch_lib = os.path.join(os.path.dirname(torch.__file__), "lib")

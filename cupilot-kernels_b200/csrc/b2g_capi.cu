@@ -798,6 +798,12 @@ int* current_error_word() {
   DeviceState* ds = nullptr;
   return device_state(&ds) == B2G_OK ? ds->err_word : nullptr;
 }
+int current_device(Device* out) {
+  DeviceState* ds = nullptr;
+  const int rc = device_state(&ds);
+  if (rc == B2G_OK) *out = Device{ds->num_sms, ds->err_word};
+  return rc;
+}
 long long current_wait_limit_ns() { return wait_limit_ns(); }
 bool pdl_enabled() { return B2G_PDL != 0; }
 }  // namespace b2g

@@ -9,6 +9,14 @@ namespace b2g {
 // sm_100 device is current.
 int* current_error_word();
 
+// The current device: its SMs and its error word.  B2G_ERR_NO_DEVICE when no
+// sm_100 device is current.
+struct Device {
+  int num_sms = 0;
+  int* error_word = nullptr;
+};
+int current_device(Device* out);
+
 // Bound on every device-side wait, in ns (B2G_WAIT_LIMIT_MS, default 2 s).
 long long current_wait_limit_ns();
 

@@ -1,0 +1,602 @@
+// b2g_prompt.cu — causal attention of packed prompts with grouped heads on
+// tcgen05 (b2g_prompt_attention).
+//
+// o_i = sum_j exp(z_ij - m_i) v_j / sum_j exp(z_ij - m_i), z = scale * q k^T,
+// in one pass over the keys: with S a tile of 128 rows by 128 keys,
+//   m' = max(m, rowmax S),  P = exp(S - m'),  l = l exp(m - m') + rowsum P,
+//   O = O exp(m - m') + P V.
+// The rows of a tile are tokens times the query heads that share a kv head
+// (row = token * group + head, one TMA box), so K and V are read once for the
+// group and a group's short prompt still fills a tile.  A CTA takes two such
+// tiles of one sequence and kv head.  S, P and O live in tensor memory: S0 S1
+// O0 O1, 128 columns each, P over the first half of its S.
+//   warps 0-3, 4-7   softmax of tile 0 / 1, a thread a row: S from tensor
+//                    memory, P back in 16 bits, at the end O / l to memory
+//   warp 8           the products: while one tile's softmax runs, the other
+//                    tile's P V and next Q K^T keep the tensor cores busy
+//   warp 9           TMA loads: Q, then K and V tiles through a ring
+// The maximum is taken over only where it grew by more than 2^8 (P stays
+// within 16 bits' range, l and O are fp32): then, rarely, the softmax warps
+// rescale O themselves.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <mutex>
+
+#include "../../include/b2g_serving.h"
+#include "b2g_internal.h"
+#include "ptx_sm100.cuh"
+
+namespace b2g {
+namespace prompt {
+
+constexpr int kRows = 128;            // rows of a tile
+constexpr int kKeys = 128;            // keys of a tile
+constexpr int kSoftmaxWarps = 8;
+constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr float kGrow = 8.f;
+constexpr uint64_t kDrainLimitNs = 100000000ull;
+constexpr int kBoxBytes = 128 * 128;  // 64 columns x 128 rows of 16 bits
+
+enum : int { kErrFull = 0x301, kErrEmpty = 0x302, kErrS = 0x303, kErrP = 0x304, kErrO = 0x305,
+             kErrQ = 0x306 };
+
+template <int DP>
+struct Smem {
+  static constexpr int kBoxes = DP / 64;
+  static constexpr int kTileBytes = kBoxes * kBoxBytes;     // a Q, K or V tile
+  static constexpr int kStages = DP == 128 ? 5 : 8;
+  static constexpr int kOffRing = 2 * kTileBytes;
+  static constexpr int kOffBars = kOffRing + kStages * kTileBytes;
+  static constexpr int kNumBars = 2 * kStages + 2 * 4 + 1;
+  static constexpr int kOffMisc = kOffBars + kNumBars * 8;
+  static constexpr int kBytes = kOffMisc + 64 + 1024;
+};
+static_assert(Smem<128>::kBytes <= 232448 && Smem<64>::kBytes <= 232448, "shared memory budget");
+
+struct Params {
+  const int32_t* cu_q;
+  const int32_t* cu_k;
+  int sequences, tokens, tokens_k, heads, kv_heads, group, dim;
+  int tile_tokens;                    // tokens of a tile: 128 / group
+  int causal;
+  int slots;                          // upper bound of tile pairs over all sequences
+  float scale_log2;
+  uint16_t* out;
+  int64_t out_token, out_head;
+  float* lse;
+  long long wait_limit_ns;
+  int* err;
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void fail(int* err, volatile int* abort, int code) {
+  atomicCAS(err, 0, code);
+  *abort = 1;
+}
+
+// D += A B with A in tensor memory (16-bit pairs, 128 lanes).
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
+      "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
+      "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() {
+  asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void tmem_wait_regs(uint32_t (&r)[32]) {
+  ptx::tmem_ld_wait();
+#pragma unroll
+  for (int i = 0; i < 32; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack(float a, float b) {
+  if (BF16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// What a CTA works on; all lengths cut to the tensors' sizes.
+struct Item {
+  int q0, qlen, k0, klen, first;      // first: token of tile 0's row 0, within the sequence
+  int head;
+};
+
+__device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// Tile pair x of all sequences: sequence s owns the places from
+// cu[s] / span + s on, at least as many as it has pairs; some stay empty.
+__device__ __forceinline__ bool find_item(const Params& p, int x, int head, Item* it) {
+  const int span = 2 * p.tile_tokens;
+  int lo = 0, hi = p.sequences;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (clampi(p.cu_q[mid], 0, p.tokens) / span + mid <= x) lo = mid;
+    else hi = mid;
+  }
+  it->head = head;
+  it->q0 = clampi(p.cu_q[lo], 0, p.tokens);
+  it->qlen = clampi(p.cu_q[lo + 1], 0, p.tokens) - it->q0;
+  it->k0 = clampi(p.cu_k[lo], 0, p.tokens_k);
+  it->klen = max(clampi(p.cu_k[lo + 1], 0, p.tokens_k) - it->k0, 0);
+  it->first = (x - it->q0 / span - lo) * span;
+  return it->first >= 0 && it->first < it->qlen;
+}
+
+// Keys that token `tok` of the sequence sees.
+__device__ __forceinline__ int keys_of(const Params& p, const Item& it, int tok) {
+  if (!p.causal) return it.klen;
+  return clampi(tok + it.klen - it.qlen + 1, 0, it.klen);
+}
+
+template <int DP, bool BF16>
+__global__ void __launch_bounds__(kThreads, 1)
+    prompt_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                  const __grid_constant__ CUtensorMap map_v, const Params p) {
+  using L = Smem<DP>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
+  uint64_t* empty = full + L::kStages;
+  uint64_t* q_full = empty + L::kStages;     // [2]
+  uint64_t* s_full = q_full + 2;             // [2] S of the tile is complete
+  uint64_t* p_ready = q_full + 4;            // [2] P of the tile is stored
+  uint64_t* o_done = q_full + 6;             // [2] P V of the tile is added to O
+  uint64_t* drain = q_full + 8;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
+  int* has_item = reinterpret_cast<int*>(smem + L::kOffMisc + 8);
+  Item* item = reinterpret_cast<Item*>(smem + L::kOffMisc + 16);
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+  // Rows of no sequence.
+  {
+    const int before = p.sequences ? clampi(p.cu_q[0], 0, p.tokens) : 0;
+    const int after = p.sequences ? clampi(p.cu_q[p.sequences], 0, p.tokens) : 0;
+    const int64_t n = static_cast<int64_t>(before + p.tokens - after) * p.heads;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < n;
+         i += static_cast<int64_t>(gridDim.x) * kThreads) {
+      int64_t t = i / p.heads;
+      const int h = static_cast<int>(i % p.heads);
+      if (t >= before) t += after - before;
+      uint16_t* o = p.out + t * p.out_token + h * p.out_head;
+      for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
+      if (p.lse) p.lse[t * p.heads + h] = -INFINITY;
+    }
+  }
+  if (tid == 0) {
+    // Late tiles see the most keys: they go first.
+    *has_item = p.sequences > 0 && find_item(p, p.slots - 1 - static_cast<int>(blockIdx.x) / p.kv_heads,
+                                             static_cast<int>(blockIdx.x) % p.kv_heads, item);
+    for (int s = 0; s < L::kStages; ++s) {
+      ptx::mbar_init(&full[s], 1);
+      ptx::mbar_init(&empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
+      ptx::mbar_init(&o_done[i], 1);
+    }
+    ptx::mbar_init(drain, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
+  __syncthreads();
+  if (!*has_item) return;
+  const Item it = *item;
+  if (warp == kSoftmaxWarps) {
+    ptx::tmem_alloc(tmem_slot, 512);
+    ptx::tmem_relinquish();
+  }
+  ptx::tc_fence_before();
+  __syncthreads();
+  ptx::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  // Key tiles of each row tile (none: the tile has no rows, or they see nothing).
+  int n_of[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int t0 = it.first + i * p.tile_tokens;
+    const int last = min(t0 + p.tile_tokens, it.qlen) - 1;
+    n_of[i] = t0 < it.qlen ? (keys_of(p, it, last) + kKeys - 1) / kKeys : 0;
+  }
+  const int n0 = n_of[0], n1 = n_of[1], n = max(n0, n1);
+
+  if (warp == kSoftmaxWarps + 1) {
+    // ------------------------------------------------------------ loads
+    if (lane == 0 && n > 0) {
+      ptx::prefetch_tmap(&map_q);
+      ptx::prefetch_tmap(&map_k);
+      ptx::prefetch_tmap(&map_v);
+      const uint32_t q_bytes = L::kBoxes * p.group * p.tile_tokens * 128;
+      auto load_q = [&](int i) {
+        ptx::mbar_arrive_expect_tx(&q_full[i], q_bytes);
+        for (int b = 0; b < L::kBoxes; ++b)
+          ptx::tma_load_3d(smem + i * L::kTileBytes + b * kBoxBytes, &map_q, &q_full[i], b * 64,
+                           it.head * p.group, it.q0 + it.first + i * p.tile_tokens);
+      };
+      int issued = 0;
+      bool ok = true;
+      auto load_kv = [&](const CUtensorMap* map, int j) {
+        const int s = issued % L::kStages;
+        if (!ptx::mbar_wait(&empty[s], ((issued / L::kStages) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+          fail(p.err, abort_flag, kErrEmpty);
+          return false;
+        }
+        ptx::mbar_arrive_expect_tx(&full[s], L::kTileBytes);
+        for (int b = 0; b < L::kBoxes; ++b)
+          ptx::tma_load_3d(smem + L::kOffRing + s * L::kTileBytes + b * kBoxBytes, map, &full[s],
+                           b * 64, it.head, it.k0 + j * kKeys);
+        ++issued;
+        return true;
+      };
+      load_q(0);
+      ok = load_kv(&map_k, 0);
+      load_q(1);
+      ok = ok && load_kv(&map_v, 0);
+      for (int j = 1; j < n && ok; ++j) ok = load_kv(&map_k, j) && load_kv(&map_v, j);
+      // Every load has landed before the CTA may leave.
+      volatile int never = 0;
+      for (int i = 0; i < 2; ++i) ptx::mbar_wait(&q_full[i], 0, &never, kDrainLimitNs);
+      for (int e = max(0, issued - L::kStages); e < issued; ++e)
+        ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
+    }
+  } else if (warp == kSoftmaxWarps) {
+    // ------------------------------------------------------------ products
+    constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+    const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
+    const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
+    const uint32_t ring = ptx::smem_addr(smem + L::kOffRing);
+    bool ok = n > 0;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+      if (!ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) {
+        if (lane == 0) fail(p.err, abort_flag, code);
+        return false;
+      }
+      ptx::tc_fence_after();
+      return true;
+    };
+    auto wait_full = [&](int e) {
+      return wait(&full[e % L::kStages], (e / L::kStages) & 1, kErrFull);
+    };
+    auto scores = [&](int i, int e) {      // S_i = Q_i K^T, K in ring entry e
+      const uint32_t sq = ptx::smem_addr(smem + i * L::kTileBytes);
+      const uint32_t sk = ring + (e % L::kStages) * L::kTileBytes;
+      for (int k = 0; k < p.dim / 16; ++k) {
+        const uint32_t at = (k >> 2) * kBoxBytes + (k & 3) * 32;
+        ptx::mma_f16(tmem + i * kKeys, ptx::smem_desc(sq + at, 16, 1024, ptx::kLayoutSw128),
+                     ptx::smem_desc(sk + at, 16, 1024, ptx::kLayoutSw128), idesc_s, k > 0);
+      }
+      ptx::mma_commit(&s_full[i]);
+    };
+    auto values = [&](int i, int e, bool add) {   // O_i += P_i V, V in ring entry e
+      const uint32_t sv = ring + (e % L::kStages) * L::kTileBytes;
+      for (int k = 0; k < kKeys / 16; ++k)
+        mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8,
+               ptx::smem_desc(sv + k * 16 * 128, kBoxBytes, 1024, ptx::kLayoutSw128), idesc_o,
+               add || k > 0);
+      ptx::mma_commit(&o_done[i]);
+    };
+    if (ok) ok = wait(&q_full[0], 0, kErrQ) && wait(&q_full[1], 0, kErrQ) && wait_full(0);
+    if (ok && lane == 0) {
+      if (n0 > 0) scores(0, 0);
+      if (n1 > 0) scores(1, 0);
+      ptx::mma_commit(&empty[0]);
+    }
+    for (int j = 0; j < n && ok; ++j) {
+      const int ek = 2 * (j + 1), ev = 2 * j + 1;
+      ok = wait_full(ev);
+      if (!ok) break;
+      if ((j + 1) * kKeys > it.klen) {
+        // Rows past the sequence hold the next one's values (or nothing): their weights are 0,
+        // but 0 * inf is not.
+        uint8_t* v = smem + L::kOffRing + (ev % L::kStages) * L::kTileBytes;
+        const int from = (it.klen - j * kKeys) * 128;
+        for (int b = 0; b < L::kBoxes; ++b)
+          for (int x = from + lane * 16; x < kBoxBytes; x += 512)
+            *reinterpret_cast<uint4*>(v + b * kBoxBytes + x) = make_uint4(0, 0, 0, 0);
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+      }
+      if (j + 1 < n) ok = wait_full(ek);
+      for (int i = 0; i < 2 && ok; ++i) {
+        const int ni = i ? n1 : n0;
+        if (j < ni) {
+          ok = wait(&p_ready[i], j & 1, kErrP);
+          if (ok && lane == 0) values(i, ev, j > 0);
+        }
+        if (ok && j + 1 < ni && lane == 0) scores(i, ek);
+      }
+      if (lane == 0) {
+        ptx::mma_commit(&empty[ev % L::kStages]);
+        if (j + 1 < n) ptx::mma_commit(&empty[ek % L::kStages]);
+      }
+      __syncwarp();
+    }
+    // No product may still write tensor memory when it is freed.
+    if (lane == 0) {
+      ptx::mma_commit(drain);
+      volatile int never = 0;
+      ptx::mbar_wait(drain, 0, &never, kDrainLimitNs);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int i = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const int ni = i ? n1 : n0;
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * 128;
+    const int t0 = it.first + i * p.tile_tokens;
+    const int tok = t0 + row / p.group, g = row % p.group;
+    const bool mine = row < p.tile_tokens * p.group && tok < it.qlen;
+    const int limit = keys_of(p, it, tok);
+    const int least = keys_of(p, it, t0);      // no row of the tile sees fewer keys
+    float m = -INFINITY, l = 0.f;              // m in log2 units
+    bool ok = true;
+    for (int j = 0; j < ni; ++j) {
+      if (!ptx::mbar_wait(&s_full[i], j & 1, abort_flag, p.wait_limit_ns)) {
+        if (lane == 0) fail(p.err, abort_flag, kErrS);
+        ok = false;
+        break;
+      }
+      ptx::tc_fence_after();
+      uint32_t s[4][32];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) tmem_wait_regs(s[c]);
+      if ((j + 1) * kKeys > least) {
+        const int seen = limit - j * kKeys;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int x = 0; x < 32; ++x)
+            if (c * 32 + x >= seen) s[c][x] = 0xff800000u;   // -infinity
+      }
+      float top = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int x = 0; x < 32; ++x) top = fmaxf(top, __uint_as_float(s[c][x]));
+      top *= p.scale_log2;
+      if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
+        const float now = fmaxf(m, top);
+        const float corr = now == m ? 1.f : exp2_fast(m - now);
+        m = now;
+        l *= corr;
+        if (j > 0) {
+          if (!ptx::mbar_wait(&o_done[i], (j - 1) & 1, abort_flag, p.wait_limit_ns)) {
+            if (lane == 0) fail(p.err, abort_flag, kErrO);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after();
+          for (int d = 0; d < p.dim; d += 32) {
+            uint32_t o[32];
+            ptx::tmem_ld_32x32b_x32(to + d, o);
+            tmem_wait_regs(o);
+#pragma unroll
+            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+            tmem_st_x32(to + d, o);
+          }
+          tmem_st_wait();
+        }
+      }
+      const float off = m == -INFINITY ? 0.f : m;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        uint32_t w[32];
+#pragma unroll
+        for (int x = 0; x < 32; ++x) {
+          const float a = exp2_fast(__uint_as_float(s[2 * c + x / 16][(2 * x) & 31]) * p.scale_log2 - off);
+          const float b = exp2_fast(__uint_as_float(s[2 * c + x / 16][(2 * x + 1) & 31]) * p.scale_log2 - off);
+          l += a + b;
+          w[x] = pack<BF16>(a, b);
+        }
+        tmem_st_x32(ts + c * 32, w);
+      }
+      tmem_st_wait();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&p_ready[i]);
+    }
+    const int64_t t = it.q0 + tok;
+    const int h = it.head * p.group + g;
+    uint16_t* out = p.out + t * p.out_token + h * p.out_head;
+    if (ok && ni > 0) {
+      if (!ptx::mbar_wait(&o_done[i], (ni - 1) & 1, abort_flag, p.wait_limit_ns)) {
+        if (lane == 0) fail(p.err, abort_flag, kErrO);
+        ok = false;
+      }
+    }
+    if (ok) {
+      ptx::tc_fence_after();
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      for (int d = 0; d < p.dim; d += 32) {
+        uint32_t o[32];
+        if (ni > 0) {
+          ptx::tmem_ld_32x32b_x32(to + d, o);
+          tmem_wait_regs(o);
+        }
+        if (mine) {
+#pragma unroll
+          for (int x = 0; x < 32; x += 8) {
+            if (d + x < p.dim) {
+              uint32_t w[4] = {0, 0, 0, 0};
+              if (limit > 0)
+#pragma unroll
+                for (int y = 0; y < 4; ++y)
+                  w[y] = pack<BF16>(__uint_as_float(o[x + 2 * y]) * inv,
+                                    __uint_as_float(o[x + 2 * y + 1]) * inv);
+              *reinterpret_cast<uint4*>(out + d + x) = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+          }
+        }
+      }
+      if (mine && p.lse)
+        p.lse[t * p.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+    }
+  }
+
+  ptx::tc_fence_before();
+  __syncthreads();
+  if (warp == kSoftmaxWarps) {
+    ptx::tc_fence_after();
+    ptx::tmem_dealloc(tmem, 512);
+  }
+}
+
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
+                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// {dim, heads, tokens} in 16 bits; a box is 64 columns of box_heads heads of
+// box_tokens tokens, rows of 128 bytes in the 128-byte swizzle.
+bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t heads, int64_t tokens,
+              int64_t head_stride, int64_t token_stride, int box_heads, int box_tokens) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return false;
+  if (heads == 1) head_stride = dim;
+  if (tokens == 1) token_stride = std::max<int64_t>(heads * dim, head_stride);
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
+                        static_cast<cuuint64_t>(tokens)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(head_stride) * 2,
+                           static_cast<cuuint64_t>(token_stride) * 2};
+  cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int DP, bool BF16>
+int launch(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, const Params& p,
+           unsigned grid, cudaStream_t stream) {
+  static thread_local int configured = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured != dev) {
+    if (cudaFuncSetAttribute(prompt_kernel<DP, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             Smem<DP>::kBytes) != cudaSuccess)
+      return B2G_ERR_LAUNCH;
+    configured = dev;
+  }
+  prompt_kernel<DP, BF16><<<grid, kThreads, Smem<DP>::kBytes, stream>>>(q, k, v, p);
+  return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
+}
+
+}  // namespace prompt
+}  // namespace b2g
+
+extern "C" int b2g_prompt_attention(const b2g_prompt_attention_desc* d, b2g_stream_t stream_handle) {
+  using namespace b2g::prompt;
+  if (!d || d->tokens < 0 || d->tokens_k < 0 || d->sequences < 0 || d->heads < 0 ||
+      d->kv_heads < 0 || d->dim <= 0 || (d->dtype != B2G_F16 && d->dtype != B2G_BF16) ||
+      !(d->scale >= 0.f))
+    return B2G_ERR_INVALID_ARG;
+  if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return B2G_ERR_INVALID_ARG;
+  if (d->tokens == 0 || d->heads == 0) return B2G_OK;
+  if (d->dim % 16 || d->dim > 128 || d->heads / d->kv_heads > kRows || d->heads > (1 << 16) ||
+      d->tokens > 0x3fffffff || d->tokens_k > 0x3fffffff || d->sequences > 0x3fffffff)
+    return B2G_ERR_UNSUPPORTED;
+  if (!d->q || !d->out || (d->sequences > 0 && !d->cu_q) || (d->tokens_k > 0 && (!d->k || !d->v)) ||
+      (!d->cu_k && d->tokens_k != d->tokens))
+    return B2G_ERR_INVALID_ARG;
+  for (int64_t s : {d->q_token_stride, d->q_head_stride, d->k_token_stride, d->k_head_stride,
+                    d->v_token_stride, d->v_head_stride, d->out_token_stride, d->out_head_stride})
+    if (s < 0 || s % 8) return B2G_ERR_UNSUPPORTED;
+  for (const void* ptr : {d->q, d->k, d->v, static_cast<const void*>(d->out)})
+    if (reinterpret_cast<uintptr_t>(ptr) % 16) return B2G_ERR_UNSUPPORTED;
+  b2g::Device dev;
+  const int rc = b2g::current_device(&dev);
+  if (rc != B2G_OK) return rc;
+  Params p;
+  p.cu_q = d->cu_q;
+  p.cu_k = d->cu_k ? d->cu_k : d->cu_q;
+  // Without a key no tile is loaded, but the maps want memory: the queries' stands in.
+  const bool no_keys = d->tokens_k == 0;
+  p.sequences = static_cast<int>(d->sequences);
+  p.tokens = static_cast<int>(d->tokens);
+  p.tokens_k = static_cast<int>(d->tokens_k);
+  p.heads = static_cast<int>(d->heads);
+  p.kv_heads = static_cast<int>(d->kv_heads);
+  p.group = p.heads / p.kv_heads;
+  p.dim = static_cast<int>(d->dim);
+  p.tile_tokens = kRows / p.group;
+  p.causal = d->causal != 0;
+  p.scale_log2 = (d->scale > 0.f ? d->scale : 1.f / std::sqrt(static_cast<float>(d->dim))) *
+                 1.4426950408889634f;
+  p.out = static_cast<uint16_t*>(d->out);
+  p.out_token = d->out_token_stride;
+  p.out_head = d->out_head_stride;
+  p.lse = d->lse;
+  p.wait_limit_ns = b2g::current_wait_limit_ns();
+  p.err = dev.error_word;
+  const int64_t slots = std::max<int64_t>(d->tokens / (2 * p.tile_tokens) + d->sequences, 1);
+  if (slots * p.kv_heads > 0x7fffffff) return B2G_ERR_UNSUPPORTED;
+  p.slots = static_cast<int>(slots);
+  const bool bf = d->dtype == B2G_BF16;
+  CUtensorMap mq, mk, mv;
+  if (!make_map(&mq, d->q, bf, d->dim, d->heads, d->tokens, d->q_head_stride, d->q_token_stride,
+                p.group, p.tile_tokens) ||
+      !make_map(&mk, no_keys ? d->q : d->k, bf, d->dim, no_keys ? 1 : d->kv_heads,
+                no_keys ? 1 : d->tokens_k, d->k_head_stride, d->k_token_stride, 1, kKeys) ||
+      !make_map(&mv, no_keys ? d->q : d->v, bf, d->dim, no_keys ? 1 : d->kv_heads,
+                no_keys ? 1 : d->tokens_k, d->v_head_stride, d->v_token_stride, 1, kKeys))
+    return B2G_ERR_UNSUPPORTED;
+  const unsigned grid = static_cast<unsigned>(slots * p.kv_heads);
+  cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
+  if (d->dim <= 64)
+    return bf ? launch<64, true>(mq, mk, mv, p, grid, stream) : launch<64, false>(mq, mk, mv, p, grid, stream);
+  return bf ? launch<128, true>(mq, mk, mv, p, grid, stream) : launch<128, false>(mq, mk, mv, p, grid, stream);
+}

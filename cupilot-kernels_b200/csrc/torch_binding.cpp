@@ -15,6 +15,7 @@
 #include <atomic>
 
 #include "../../include/b2g_gemm.h"
+#include "../../include/b2g_serving.h"
 
 namespace {
 
@@ -471,6 +472,282 @@ at::Tensor splitk_peer_matmul(at::Tensor A, at::Tensor B, std::vector<int64_t> m
   return C;
 }
 
+// ------------------------------------------------------------------ serving
+// The paged 8-bit cache (include/b2g_serving.h).  The tensors' shapes, types
+// and devices are checked here; lengths, tables and slots stay on the device
+// and the kernels bound what they form from them.
+
+int dtype_of(const at::Tensor& t, const char* name) {
+  const auto dt = t.scalar_type();
+  TORCH_CHECK(dt == at::kHalf || dt == at::kBFloat16, name, " must be float16 or bfloat16");
+  return dt == at::kHalf ? B2G_F16 : B2G_BF16;
+}
+
+void check_ints(const at::Tensor& t, const char* name, int64_t dims, at::ScalarType dt,
+                const at::Tensor& like) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the same CUDA device");
+  TORCH_CHECK(t.scalar_type() == dt, name, " must be ", dt);
+  TORCH_CHECK(t.dim() == dims, name, " must be ", dims, "-D");
+  TORCH_CHECK(t.is_contiguous(), name, " must be contiguous");
+}
+
+// (rows, heads, dim) as the kernels read it: dim contiguous, 16-byte rows.
+// Views of a larger tensor (a slice of a fused projection, a transposed
+// layout) are read in place; anything else is copied.
+at::Tensor rows_of(const at::Tensor& t) {
+  bool fine = t.size(2) <= 1 || t.stride(2) == 1;
+  for (int i = 0; i < 2; ++i)
+    if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8)) fine = false;
+  if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) fine = false;
+  return fine ? t : t.contiguous();
+}
+// A stride that is never stepped may hold anything: make it one the kernels take.
+int64_t stride_of(const at::Tensor& t, int i) {
+  return t.size(i) > 1 ? t.stride(i) : (i == 0 ? t.size(1) * t.size(2) : t.size(2));
+}
+
+struct Cache {
+  int codes;
+  int64_t blocks, heads, block_size, dim;
+};
+
+Cache check_cache(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ks,
+                  const at::Tensor& vs, const at::Tensor& like) {
+  TORCH_CHECK(kc.dim() == 4, "k_cache must be (blocks, kv_heads, block_size, dim)");
+  TORCH_CHECK(vc.sizes() == kc.sizes(), "k_cache and v_cache must have one shape");
+  const auto dt = kc.scalar_type();
+  TORCH_CHECK(dt == at::kChar || dt == at::kFloat8_e4m3fn, "k_cache must be int8 or float8_e4m3fn");
+  TORCH_CHECK(vc.scalar_type() == dt, "k_cache and v_cache must have one dtype");
+  for (const auto* t : {&kc, &vc, &ks, &vs}) {
+    TORCH_CHECK(t->is_cuda() && t->device() == like.device(),
+                "the cache and its scales must be on the same CUDA device");
+    TORCH_CHECK(t->is_contiguous(), "the cache and its scales must be contiguous");
+  }
+  for (const auto* t : {&ks, &vs}) {
+    TORCH_CHECK(t->scalar_type() == at::kFloat, "k_scale and v_scale must be float32");
+    TORCH_CHECK(t->dim() == 2 && t->size(0) == kc.size(0) && t->size(1) == kc.size(1),
+                "k_scale and v_scale must be (blocks, kv_heads)");
+  }
+  const int64_t bs = kc.size(2), d = kc.size(3);
+  TORCH_CHECK(bs >= 16 && bs <= 256 && (bs & (bs - 1)) == 0,
+              "block_size must be a power of two from 16 to 256, got ", bs);
+  TORCH_CHECK(d > 0 && d % 16 == 0 && d <= 128, "dim must be a multiple of 16, at most 128, got ", d);
+  return {dt == at::kChar ? B2G_I8 : B2G_E4M3, kc.size(0), kc.size(1), bs, d};
+}
+
+std::vector<at::Tensor> block_tables(const at::Tensor& context_lens, const at::Tensor& new_lens,
+                                     const at::Tensor& block_table, const at::Tensor& free_blocks,
+                                     const at::Tensor& free_count, int64_t total_tokens,
+                                     int64_t block_size) {
+  check_ints(context_lens, "context_lens", 1, at::kInt, context_lens);
+  check_ints(new_lens, "new_lens", 1, at::kInt, context_lens);
+  check_ints(free_blocks, "free_blocks", 1, at::kInt, context_lens);
+  check_ints(free_count, "free_count", 1, at::kInt, context_lens);
+  const int64_t n = context_lens.size(0);
+  TORCH_CHECK(new_lens.size(0) == n, "new_lens must have one value for each request");
+  TORCH_CHECK(free_count.size(0) == 1, "free_count must have one value");
+  TORCH_CHECK(block_table.is_cuda() && block_table.device() == context_lens.device() &&
+                  block_table.scalar_type() == at::kInt && block_table.dim() == 2,
+              "block_table must be a 2-D int32 tensor on the same CUDA device");
+  TORCH_CHECK(block_table.size(0) == n, "block_table must have one row for each request");
+  TORCH_CHECK(block_table.size(1) <= 1 || block_table.stride(1) == 1,
+              "block_table's rows must be contiguous");
+  TORCH_CHECK(n <= 1 || block_table.stride(0) >= block_table.size(1),
+              "block_table's rows must not overlap");
+  TORCH_CHECK(total_tokens >= 0, "total_tokens must not be negative");
+  TORCH_CHECK(block_size >= 16 && block_size <= 256 && (block_size & (block_size - 1)) == 0,
+              "block_size must be a power of two from 16 to 256, got ", block_size);
+  TORCH_CHECK(n <= B2G_MAX_TABLE_REQUESTS, "at most ", B2G_MAX_TABLE_REQUESTS, " requests");
+  const c10::cuda::CUDAGuard guard(context_lens.device());
+  at::Tensor slots = at::empty({total_tokens}, context_lens.options().dtype(at::kLong));
+  at::Tensor cu = at::empty({n + 1}, context_lens.options());
+  at::Tensor lens = at::empty({n}, context_lens.options());
+  at::Tensor left = at::empty({1}, context_lens.options());
+  auto stream = at::cuda::getCurrentCUDAStream(context_lens.device().index());
+  check_status(
+      b2g_block_tables(context_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n,
+                       block_table.data_ptr<int32_t>(), block_table.size(1),
+                       n > 1 ? block_table.stride(0) : block_table.size(1),
+                       free_blocks.data_ptr<int32_t>(), free_blocks.size(0),
+                       free_count.data_ptr<int32_t>(), total_tokens, static_cast<int>(block_size),
+                       slots.data_ptr<int64_t>(), cu.data_ptr<int32_t>(), lens.data_ptr<int32_t>(),
+                       left.data_ptr<int32_t>(), stream.stream()),
+      "b2g_block_tables");
+  return {slots, cu, lens, left};
+}
+
+void cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& slots,
+                  const at::Tensor& k_cache, const at::Tensor& v_cache, const at::Tensor& k_scale,
+                  const at::Tensor& v_scale) {
+  TORCH_CHECK(k.is_cuda() && k.dim() == 3, "k must be a CUDA tensor (tokens, kv_heads, dim)");
+  TORCH_CHECK(v.is_cuda() && v.device() == k.device() && v.sizes() == k.sizes() &&
+                  v.scalar_type() == k.scalar_type(),
+              "k and v must have one shape, dtype and device");
+  b2g_cache_append_desc d{};
+  d.dtype = dtype_of(k, "k and v");
+  const Cache c = check_cache(k_cache, v_cache, k_scale, v_scale, k);
+  TORCH_CHECK(k.size(1) == c.heads && k.size(2) == c.dim, "k is ", k.sizes(), ", the cache holds ",
+              c.heads, " heads of ", c.dim);
+  check_ints(slots, "slots", 1, at::kLong, k);
+  TORCH_CHECK(slots.size(0) == k.size(0), "slots must have one value for each token");
+  if (k.numel() == 0) return;
+  const c10::cuda::CUDAGuard guard(k.device());
+  const at::Tensor kr = rows_of(k), vr = rows_of(v);
+  d.codes = c.codes;
+  d.tokens = k.size(0);
+  d.kv_heads = c.heads;
+  d.dim = c.dim;
+  d.num_blocks = c.blocks;
+  d.block_size = c.block_size;
+  d.k = kr.data_ptr();
+  d.k_token_stride = stride_of(kr, 0);
+  d.k_head_stride = stride_of(kr, 1);
+  d.v = vr.data_ptr();
+  d.v_token_stride = stride_of(vr, 0);
+  d.v_head_stride = stride_of(vr, 1);
+  d.slots = slots.data_ptr<int64_t>();
+  d.k_cache = k_cache.data_ptr();
+  d.v_cache = v_cache.data_ptr();
+  d.k_scale = k_scale.data_ptr<float>();
+  d.v_scale = v_scale.data_ptr<float>();
+  auto stream = at::cuda::getCurrentCUDAStream(k.device().index());
+  check_status(b2g_cache_append(&d, stream.stream()), "b2g_cache_append");
+}
+
+float scale_of(c10::optional<double> scale) {
+  if (!scale.has_value()) return 0.f;
+  TORCH_CHECK(*scale > 0, "scale must be positive");
+  return static_cast<float>(*scale);
+}
+
+// The output, with its log sums where asked for.
+py::object with_lse(const at::Tensor& out, const at::Tensor& lse, bool both) {
+  if (both) return py::cast(std::make_pair(out, lse));
+  return py::cast(out);
+}
+
+py::object cache_attention(const at::Tensor& q, const at::Tensor& k_cache, const at::Tensor& v_cache,
+                           const at::Tensor& k_scale, const at::Tensor& v_scale,
+                           const at::Tensor& block_table, const at::Tensor& seq_lens,
+                           c10::optional<double> scale, bool return_lse) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, "q must be a CUDA tensor (requests, heads, dim)");
+  b2g_cache_attention_desc d{};
+  d.dtype = dtype_of(q, "q");
+  const Cache c = check_cache(k_cache, v_cache, k_scale, v_scale, q);
+  const int64_t n = q.size(0), heads = q.size(1);
+  TORCH_CHECK(q.size(2) == c.dim, "q has dim ", q.size(2), ", the cache ", c.dim);
+  TORCH_CHECK(heads == 0 || (c.heads > 0 && heads % c.heads == 0),
+              "q's heads must be a multiple of the cache's");
+  TORCH_CHECK(block_table.is_cuda() && block_table.device() == q.device() &&
+                  block_table.scalar_type() == at::kInt && block_table.dim() == 2,
+              "block_table must be a 2-D int32 tensor on the same CUDA device");
+  TORCH_CHECK(block_table.size(0) == n, "block_table must have one row for each request");
+  TORCH_CHECK(block_table.size(1) <= 1 || block_table.stride(1) == 1,
+              "block_table's rows must be contiguous");
+  TORCH_CHECK(n <= 1 || block_table.stride(0) >= block_table.size(1),
+              "block_table's rows must not overlap");
+  check_ints(seq_lens, "seq_lens", 1, at::kInt, q);
+  TORCH_CHECK(seq_lens.size(0) == n, "seq_lens must have one value for each request");
+  d.scale = scale_of(scale);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({n, heads}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return with_lse(out, lse, return_lse);
+  const at::Tensor qr = rows_of(q);
+  d.codes = c.codes;
+  d.requests = n;
+  d.heads = heads;
+  d.kv_heads = c.heads;
+  d.dim = c.dim;
+  d.num_blocks = c.blocks;
+  d.block_size = c.block_size;
+  d.q = qr.data_ptr();
+  d.q_row_stride = stride_of(qr, 0);
+  d.q_head_stride = stride_of(qr, 1);
+  d.k_cache = k_cache.data_ptr();
+  d.v_cache = v_cache.data_ptr();
+  d.k_scale = k_scale.data_ptr<float>();
+  d.v_scale = v_scale.data_ptr<float>();
+  d.block_table = block_table.data_ptr<int32_t>();
+  d.table_width = block_table.size(1);
+  d.table_ld = n > 1 ? block_table.stride(0) : block_table.size(1);
+  d.seq_lens = seq_lens.data_ptr<int32_t>();
+  d.out = out.data_ptr();
+  d.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+  const int64_t ws = b2g_cache_attention_workspace_bytes(&d);
+  TORCH_CHECK(ws >= 0, "b2g: cache attention beyond the supported sizes");
+  const at::Tensor wst = at::empty({ws}, q.options().dtype(at::kByte));
+  d.workspace = wst.data_ptr();
+  d.workspace_bytes = ws;
+  auto stream = at::cuda::getCurrentCUDAStream(q.device().index());
+  check_status(b2g_cache_attention(&d, stream.stream()), "b2g_cache_attention");
+  return with_lse(out, lse, return_lse);
+}
+
+py::object prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                            const at::Tensor& cu_seqlens, c10::optional<at::Tensor> cu_seqlens_k,
+                            bool causal, c10::optional<double> scale, bool return_lse) {
+  TORCH_CHECK(q.is_cuda() && q.dim() == 3, "q must be a CUDA tensor (tokens, heads, dim)");
+  TORCH_CHECK(k.dim() == 3 && v.sizes() == k.sizes(),
+              "k and v must be (tokens, kv_heads, dim) of one shape");
+  b2g_prompt_attention_desc d{};
+  d.dtype = dtype_of(q, "q, k and v");
+  for (const auto* t : {&k, &v}) {
+    TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "q, k and v must be on the same device");
+    TORCH_CHECK(t->scalar_type() == q.scalar_type(), "q, k and v must have one dtype");
+  }
+  const int64_t heads = q.size(1), kv_heads = k.size(1), dim = q.size(2);
+  TORCH_CHECK(k.size(2) == dim, "q has dim ", dim, ", k and v ", k.size(2));
+  TORCH_CHECK(dim > 0 && dim % 16 == 0 && dim <= 128,
+              "dim must be a multiple of 16, at most 128, got ", dim);
+  TORCH_CHECK(heads == 0 || (kv_heads > 0 && heads % kv_heads == 0),
+              "q's heads must be a multiple of k's");
+  TORCH_CHECK(heads == 0 || heads / kv_heads <= 128, "at most 128 query heads to a kv head");
+  check_ints(cu_seqlens, "cu_seqlens", 1, at::kInt, q);
+  TORCH_CHECK(cu_seqlens.size(0) >= 1, "cu_seqlens must have a value more than sequences");
+  const bool own_k = cu_seqlens_k.has_value() && cu_seqlens_k->defined();
+  if (own_k) {
+    check_ints(*cu_seqlens_k, "cu_seqlens_k", 1, at::kInt, q);
+    TORCH_CHECK(cu_seqlens_k->size(0) == cu_seqlens.size(0),
+                "cu_seqlens_k must have as many values as cu_seqlens");
+  } else {
+    TORCH_CHECK(k.size(0) == q.size(0), "k must have q's tokens where cu_seqlens_k is not given");
+  }
+  d.scale = scale_of(scale);
+  const c10::cuda::CUDAGuard guard(q.device());
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor lse;
+  if (return_lse) lse = at::empty({q.size(0), heads}, q.options().dtype(at::kFloat));
+  if (out.numel() == 0) return with_lse(out, lse, return_lse);
+  const at::Tensor qr = rows_of(q), kr = rows_of(k), vr = rows_of(v);
+  d.causal = causal;
+  d.tokens = q.size(0);
+  d.tokens_k = k.size(0);
+  d.sequences = cu_seqlens.size(0) - 1;
+  d.heads = heads;
+  d.kv_heads = kv_heads;
+  d.dim = dim;
+  d.q = qr.data_ptr();
+  d.q_token_stride = stride_of(qr, 0);
+  d.q_head_stride = stride_of(qr, 1);
+  d.k = kr.data_ptr();
+  d.k_token_stride = stride_of(kr, 0);
+  d.k_head_stride = stride_of(kr, 1);
+  d.v = vr.data_ptr();
+  d.v_token_stride = stride_of(vr, 0);
+  d.v_head_stride = stride_of(vr, 1);
+  d.out = out.data_ptr();
+  d.out_token_stride = heads * dim;
+  d.out_head_stride = dim;
+  d.cu_q = cu_seqlens.data_ptr<int32_t>();
+  d.cu_k = own_k ? cu_seqlens_k->data_ptr<int32_t>() : nullptr;
+  d.lse = return_lse ? lse.data_ptr<float>() : nullptr;
+  auto stream = at::cuda::getCurrentCUDAStream(q.device().index());
+  check_status(b2g_prompt_attention(&d, stream.stream()), "b2g_prompt_attention");
+  return with_lse(out, lse, return_lse);
+}
+
 int64_t read_device_error(int64_t device) {
   int32_t code = 0;
   check_status(b2g_read_device_error(static_cast<int>(device), &code), "b2g_read_device_error");
@@ -511,6 +788,17 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("set_thread_precision", &set_thread_precision);
   m.def("get_thread_precision", &get_thread_precision);
   m.def("read_device_error", &read_device_error);
+  m.def("block_tables", &block_tables, py::arg("context_lens"), py::arg("new_lens"),
+        py::arg("block_table"), py::arg("free_blocks"), py::arg("free_count"),
+        py::arg("total_tokens"), py::arg("block_size"));
+  m.def("cache_append", &cache_append, py::arg("k"), py::arg("v"), py::arg("slots"),
+        py::arg("k_cache"), py::arg("v_cache"), py::arg("k_scale"), py::arg("v_scale"));
+  m.def("cache_attention", &cache_attention, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"),
+        py::arg("k_scale"), py::arg("v_scale"), py::arg("block_table"), py::arg("seq_lens"),
+        py::arg("scale") = py::none(), py::arg("return_lse") = false);
+  m.def("prompt_attention", &prompt_attention, py::arg("q"), py::arg("k"), py::arg("v"),
+        py::arg("cu_seqlens"), py::arg("cu_seqlens_k") = py::none(), py::arg("causal") = true,
+        py::arg("scale") = py::none(), py::arg("return_lse") = false);
   m.def("splitk_peer_reduce", &splitk_peer_reduce, "one epoch of the cross-GPU K-split sum");
   m.def("splitk_peer_matmul", &splitk_peer_matmul,
         "this rank's K-slice product and the cross-GPU sum, one kernel");

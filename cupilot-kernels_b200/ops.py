@@ -144,6 +144,73 @@ read_device_error = _ext.read_device_error
 
 batched_matmul_out = _ext.batched_matmul_out
 
+# ---------------------------------------------------------------- serving
+# The operators of a paged 8-bit key/value cache (`serving.PagedCache` runs
+# them together).  All of them work on the current stream and neither
+# synchronise nor read a device value on the host; lengths, tables and slots
+# are int32 / int64 CUDA tensors.
+
+
+def block_tables(context_lens, new_lens, block_table, free_blocks, free_count, total_tokens,
+                 block_size):
+    """Block tables, slot map and row offsets of one serving step.
+
+    Request r holds `context_lens[r]` tokens and gains `new_lens[r]`; the
+    blocks that it lacks are taken from the top of the stack
+    `free_blocks[:free_count]`, the requests in order, and written into its
+    row of `block_table` (requests, width), in place.  `total_tokens`, the
+    sum of `new_lens`, is known on the host (the step's rows).
+
+    Returns `(slots, cu_seqlens, seq_lens, free_count)`: each new token's
+    place in the cache (int64, -1: none), the new tokens before each request
+    (requests + 1), the lengths after the step, and what is left of the
+    stack (below 0: that many blocks were missing).
+    """
+    return tuple(_ext.block_tables(context_lens, new_lens, block_table, free_blocks, free_count,
+                                   total_tokens, block_size))
+
+
+def cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale):
+    """Quantise keys and values (tokens, kv_heads, dim), fp16 or bf16, into
+    the cache, in place.
+
+    `k_cache`, `v_cache`: (blocks, kv_heads, block_size, dim) int8 or
+    float8_e4m3fn; `k_scale`, `v_scale`: (blocks, kv_heads) float32, one
+    scale for each block of tokens and head.  A scale grows with what is
+    added to its block, whose earlier codes are rounded to it.  The tokens of
+    one block stand together, in order (as `block_tables` places them).
+    """
+    _ext.cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale)
+
+
+def cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale=None,
+                    return_lse=False):
+    """softmax(scale q K^T) V for one query token of each request over its
+    cached tokens: q (requests, heads, dim), heads a multiple of the cache's;
+    scale defaults to 1/sqrt(dim).  A request of length 0 gives zeros.
+
+    Returns the output in q's dtype, with `return_lse` also the natural
+    logarithms of the softmax sums (requests, heads), float32.
+    """
+    return _ext.cache_attention(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, scale,
+                                return_lse)
+
+
+def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=None,
+                     return_lse=False):
+    """Attention of whole prompts packed one after another: q (tokens, heads,
+    dim), k and v (tokens, kv_heads, dim), fp16 or bf16, sequence s in rows
+    `cu_seqlens[s]` to `cu_seqlens[s + 1]`.
+
+    `cu_seqlens_k` gives keys their own rows (a chunk of a longer prompt:
+    the last query sees the last key).  A query that sees no key gives zeros.
+
+    Returns the output in q's dtype, with `return_lse` also the natural
+    logarithms of the softmax sums (tokens, heads), float32.
+    """
+    return _ext.prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, return_lse)
+
+
 _HOST_STREAMS = {}
 
 
