@@ -4,18 +4,22 @@
 // out[j] = sum_n exp(z_n - max z) V_n / sum_n exp(z_n - max z),
 // z_n = scale * q_j . K_n, one pass over K and V with the running maximum and
 // sum.  With c the codes and a scale for each block and head, z_n = (scale *
-// kscale) * (q . c_n), and the products run on the codes: int8 and e4m3 are
-// exact in fp16, so a warp's m16n8k16 product takes q (16 rows: the query
-// heads that share the kv head) against 16 tokens' codes widened in
-// registers.  q is brought to [-1, 1] by a power of two (exact in fp16, where
-// the row's small values may go subnormal), the weights are <= 2^12 in fp16,
-// sums, maxima and the output are fp32.
+// kscale) * (q . c_n), and the products run on the codes, which fp16 holds
+// exactly: a warp's m16n8k16 products take 16 tokens' codes, widened in
+// registers, as the 16 rows and up to 8 (or 2 x 8) of the query heads that
+// share the kv head as the columns, S^T = K Q^T and O^T = V^T P^T, so that a
+// group of 8 heads fills a product.  q is brought to [-1, 1] by a power of two
+// (exact in fp16, where a row's small values may go subnormal), the weights
+// are <= 2^12 in fp16, sums, maxima and the output are fp32.
 //
-// Bound by memory: 2 * dim bytes a token and kv head, read once by 16-byte
-// loads into registers one step ahead of their use.  The (request, head,
-// 64-token) tiles are laid end to end and cut into equal ranges, one a CTA,
-// so ragged lengths fill the GPU evenly; what a cut divides is joined by a
-// second small kernel.
+// Bound by memory: 2 * dim bytes a token and kv head.  A producer warp keeps
+// a ring of 64-token stages filled by TMA (boxes of whole rows of a block in
+// the 128-byte swizzle, which the fragments' 16-byte shared loads read
+// without bank conflicts), with the blocks' scales beside them; four consumer
+// warps take 16 tokens each of every stage.  The (request, head, 64-token)
+// tiles are laid end to end and cut into equal ranges, one a CTA, so ragged
+// lengths fill the GPU evenly; what a cut divides is joined by a second small
+// kernel.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -30,26 +34,44 @@
 
 namespace {
 
+namespace ptx = b2g::ptx;
+
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kTile = 16 * kWarps;     // tokens of a CTA's step, 16 a warp
-// By the registers that a warp's state and its two steps take.
-constexpr int ctas_per_sm(int dp, int rows) { return dp == 64 ? (rows == 8 ? 5 : 4) : (rows == 8 ? 3 : 2); }
+constexpr int kWarps = 4;                       // consumers
+constexpr int kThreads = (kWarps + 1) * 32;     // and the producer
+constexpr int kTile = 16 * kWarps;              // tokens of a stage, 16 a consumer warp
 constexpr float kGrow = 8.f;           // a maximum may be passed by 2^8 before the sums are rescaled
+constexpr uint64_t kDrainLimitNs = 100000000ull;
+constexpr uint32_t kNoBlock = 0xffffffffu;   // in the place of a key scale
+enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
+
+// Shared memory of a CTA: the ring, the stages' scales, the barriers, and the
+// four warps' results of a segment.
+template <int DP, int ROWS>
+struct Smem {
+  static constexpr int kStages = DP == 128 ? 3 : 6;
+  static constexpr int kSideBytes = kTile * DP;             // K or V of a stage
+  static constexpr int kStageBytes = 2 * kSideBytes;
+  static constexpr int kOffScales = kStages * kStageBytes;  // [stage][piece]{k scale, v scale}
+  static constexpr int kOffBars = kOffScales + kStages * kWarps * 8;
+  static constexpr int kOffMisc = kOffBars + 2 * kStages * 8;
+  static constexpr int kOffJoin = kOffMisc + 64;            // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
+  static constexpr int kOffO = kOffJoin + 2 * kWarps * ROWS * 4;
+  static constexpr int kBytes = kOffO + kWarps * ROWS * DP * 4 + 1024;
+  static constexpr int kCtas = ROWS == 8 ? 3 : 2;           // a multiprocessor
+};
 
 struct Args {
   const void* q;
   int64_t q_row, q_head;
-  const uint8_t* k_cache;
-  const uint8_t* v_cache;
   const float* k_scale;
   const float* v_scale;
   const int32_t* table;
   int64_t width, ld;
   const int32_t* seq_lens;
   int requests, kv_heads, group, row_groups, dim, lg_block, bf16;
+  int box_rows;                  // rows of a TMA box: the part of a block that a stage holds
   int64_t num_blocks;
   float scale_log2;
   void* out;
@@ -60,6 +82,8 @@ struct Args {
   float* part_l;
   float* part_o;
   int grid;
+  long long wait_limit_ns;
+  int* err;
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {
@@ -76,26 +100,26 @@ __device__ __forceinline__ int tiles_of(const Args& a, int r) {
   return (length_of(a, r) + kTile - 1) / kTile;
 }
 
-__device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2,
-                                          uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                          uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// The same with rows 8-15 of A zero: their sums are neither kept nor read.
-__device__ __forceinline__ void mma_16816(float (&d)[2], uint32_t a0, uint32_t, uint32_t a2,
-                                          uint32_t, uint32_t b0, uint32_t b1) {
-  asm("{\n\t.reg .f32 x, y;\n\t"
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,x,y}, {%2,%3,%4,%3}, {%5,%6}, "
-      "{%0,%1,%7,%7};\n\t}"
-      : "+f"(d[0]), "+f"(d[1])
-      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// Four codes to two fp16 pairs.  int8: with the sign bit flipped a byte u is
-// 128 + c, and the fp16 with bits 0x6400 | u is 1024 + u, exactly.
-template <bool E4M3>
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// 1152 + c for an int8 code c, as the fp16 with bits 0x6400 | (c + 128) is 1024 + (c + 128).
+constexpr float kI8Offset = 1152.f;
+
+// Four codes to two fp16 pairs.  OFFSET: int8 codes come as 1152 + c (and the
+// caller takes the 1152 out of the sum).
+template <bool E4M3, bool OFFSET>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (E4M3) {
     asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\t"
@@ -104,220 +128,199 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
         : "r"(w));
   } else {
     const uint32_t u = w ^ 0x80808080u;
-    const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
-    uint32_t x = __byte_perm(u, 0x64646464u, 0x4140), y = __byte_perm(u, 0x64646464u, 0x4342);
-    __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&x), off);
-    __half2 hy = __hsub2(*reinterpret_cast<__half2*>(&y), off);
-    lo = *reinterpret_cast<uint32_t*>(&hx);
-    hi = *reinterpret_cast<uint32_t*>(&hy);
-  }
-}
-
-__device__ __forceinline__ uint4 load16(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-__device__ __forceinline__ uint2 load8(const uint8_t* p) {
-  uint2 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
-  return v;
-}
-
-// One warp's 16 tokens of one head.  Lane (g, c) = (lane / 4, lane % 4) holds
-// of K, for tokens g and 8 + g, the dims 64 j + 16 c .. + 15 (the k index of
-// a product may be any order of the dims that q has too), and of V, for the
-// tokens 2c, 2c+1, 2c+8, 2c+9 that it needs as pairs, DP / 8 dims from
-// DP / 8 * g (its n index, in any order that the output is read back in).
-template <int DP>
-struct Step {
-  uint4 k[2][DP / 64];
-  uint32_t v[4][DP / 32];
-  float ks, vs;
-  bool bad;
-};
-
-template <int DP>
-__device__ __forceinline__ void load_step(Step<DP>& f, const Args& a, int head, int id, int off,
-                                          int lane) {
-  const int g = lane >> 2, c = lane & 3;
-  f.bad = static_cast<uint32_t>(id) >= a.num_blocks;
-  const int64_t bh = static_cast<int64_t>(f.bad ? 0 : id) * a.kv_heads + head;
-  const int64_t at = ((bh << a.lg_block) + off) * a.dim;
-  const uint8_t* kp = a.k_cache + at;
-  const uint8_t* vp = a.v_cache + at;
-  f.ks = __ldg(a.k_scale + bh);
-  f.vs = __ldg(a.v_scale + bh);
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
-      const int d = 64 * j + 16 * c;
-      f.k[t][j] = d < a.dim ? load16(kp + (8 * t + g) * a.dim + d) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int tok = 2 * c + (t & 1) + (t >> 1) * 8;
-    const int d = DP / 8 * g;
-    const uint8_t* p = vp + tok * a.dim + d;
-    if (DP == 128) {
-      const uint4 w = d < a.dim ? load16(p) : make_uint4(0, 0, 0, 0);
-      f.v[t][0] = w.x, f.v[t][1] = w.y, f.v[t][DP / 32 - 2] = w.z, f.v[t][DP / 32 - 1] = w.w;
-    } else {
-      const uint2 w = d < a.dim ? load8(p) : make_uint2(0, 0);
-      f.v[t][0] = w.x, f.v[t][1] = w.y;
+    lo = __byte_perm(u, 0x64646464u, 0x4140);
+    hi = __byte_perm(u, 0x64646464u, 0x4342);
+    if (!OFFSET) {
+      const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
+      const __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&lo), off);
+      const __half2 hy = __hsub2(*reinterpret_cast<__half2*>(&hi), off);
+      lo = *reinterpret_cast<const uint32_t*>(&hx);
+      hi = *reinterpret_cast<const uint32_t*>(&hy);
     }
   }
 }
 
-// The warp's running state: row g (and 8 + g with ROWS == 16).
+// A warp's running state.  Lane (g, c) = (lane / 4, lane % 4).
 template <int DP, int ROWS>
 struct State {
-  static constexpr int H = ROWS / 8;
-  uint32_t q[DP / 16][2 * H];
-  float rf[H];        // scale * log2(e) * the power of two that q was divided by
-  float m[H], l[H];   // maximum so far (log2 units), this lane's part of the sum
-  float unit, per;    // o is in units of `unit` (a block's value scale), per = 1 / unit
-  float o[DP / 8][2 * H];
+  static constexpr int N = ROWS / 8;   // columns of 8 query heads
+  uint32_t q[N][DP / 16][2];           // head 8 n + g, the lane's dims
+  // Of heads 8 n + 2 c, 8 n + 2 c + 1:
+  float rf[N][2];                      // scale * log2(e) * the power of two that q was divided by
+  float start[N][2];                   // what S starts from: the int8 offset's share
+  float m[N][2], l[N][2];              // maximum so far (log2 units), this lane's part of the sum
+  float unit, per;                     // o is in units of `unit` (a block's value scale), per = 1 / unit
+  float o[N][DP / 16][4];              // dims DP/8 g + 2 t, + 1 (index / 2) of those heads (index % 2)
 };
 
+// One warp's 16 tokens.  k, v: their rows in shared memory, swizzled.
 template <int DP, int ROWS, bool E4M3>
-__device__ __forceinline__ void compute_step(State<DP, ROWS>& s, Step<DP>& f, int left, int lane) {
-  constexpr int H = ROWS / 8;
-  const int c = lane & 3;
-  float z[2][2 * H];
+__device__ __forceinline__ void compute_piece(State<DP, ROWS>& s, const uint8_t* k, const uint8_t* v,
+                                              float ks, float vs, int left, int lane) {
+  constexpr int N = ROWS / 8;
+  constexpr int kChunk = DP == 128 ? 8 : 4;      // 16-byte chunks of a row
+  const int g = lane >> 2, c = lane & 3;
+  // Chunk `at` of a row, in the 128-byte (64-byte) swizzle: XOR of row % 8 ((row / 2) % 4).
+  auto place = [&](int row, int at) {
+    return row * DP + ((at ^ (DP == 128 ? row & 7 : (row >> 1) & 3)) << 4);
+  };
+  float z[N][4];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) {
+  for (int n = 0; n < N; ++n) {
+    z[n][0] = z[n][2] = s.start[n][0];
+    z[n][1] = z[n][3] = s.start[n][1];
+  }
 #pragma unroll
-    for (int i = 0; i < 2 * H; ++i) z[t][i] = 0.f;
+  for (int j = 0; j < DP / 64; ++j) {
+    const int at = kChunk / 4 * c + j;
+    const uint4 x = *reinterpret_cast<const uint4*>(k + place(g, at));
+    const uint4 y = *reinterpret_cast<const uint4*>(k + place(g + 8, at));
+    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
-      const uint32_t w[4] = {f.k[t][j].x, f.k[t][j].y, f.k[t][j].z, f.k[t][j].w};
+    for (int i = 0; i < 4; ++i) {
+      uint32_t a[4];
+      widen4<E4M3, true>(xs[i], a[0], a[2]);
+      widen4<E4M3, true>(ys[i], a[1], a[3]);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t b0, b1;
-        widen4<E4M3>(w[i], b0, b1);
-        const uint32_t* qa = s.q[4 * j + i];
-        mma_16816(z[t], qa[0], H == 2 ? qa[H - 1] : 0u, qa[H], H == 2 ? qa[2 * H - 1] : 0u, b0, b1);
-      }
+      for (int n = 0; n < N; ++n) mma_16816(z[n], a, s.q[n][4 * j + i][0], s.q[n][4 * j + i][1]);
     }
   }
-  if (left < 16 || f.bad) {            // the last tokens, or a block outside the cache
+  // V: tokens 2c, 2c+1, 2c+8, 2c+9, dims DP/8 g ... of each.
+  uint32_t w[4][DP / 32];
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
-#pragma unroll
-      for (int i = 0; i < 2 * H; ++i)
-        if (f.bad || 8 * t + 2 * c + (i & 1) >= left) z[t][i] = -INFINITY;
-    // What is not a token's may hold anything: 0 * NaN must not reach the sums.
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-      if (f.bad || 2 * c + (t & 1) + (t >> 1) * 8 >= left)
-#pragma unroll
-        for (int j = 0; j < DP / 32; ++j) f.v[t][j] = 0;
-    if (f.bad) f.vs = 0.f, f.ks = 0.f;
+  for (int t = 0; t < 4; ++t) {
+    const int row = 2 * c + (t & 1) + (t >> 1) * 8;
+    if (DP == 128) {
+      const uint4 x = *reinterpret_cast<const uint4*>(v + place(row, g));
+      w[t][0] = x.x, w[t][1] = x.y, w[t][DP / 32 - 2] = x.z, w[t][DP / 32 - 1] = x.w;
+    } else {
+      const uint2 x = *reinterpret_cast<const uint2*>(v + place(row, g >> 1) + (g & 1) * 8);
+      w[t][0] = x.x, w[t][1] = x.y;
+    }
   }
-  float top[H];
-  bool grow = f.vs > 16.f * s.unit;
+  float top[N][2];
+  bool grow = fabsf(vs) > 16.f * s.unit;
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    const float r = s.rf[h] * f.ks;
+  for (int n = 0; n < N; ++n)
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int h = 0; h < 2; ++h) {
+      const float r = s.rf[n][h] * ks;
+      z[n][h] *= r;
+      z[n][2 + h] *= r;
+    }
+  if (left < 16) {                       // the last tokens
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        float& x = z[t][2 * h + i];
-        x = x == -INFINITY ? x : x * r;
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (g >= left) z[n][h] = -INFINITY;
+        if (g + 8 >= left) z[n][2 + h] = -INFINITY;
       }
-    top[h] = fmaxf(fmaxf(z[0][2 * h], z[0][2 * h + 1]), fmaxf(z[1][2 * h], z[1][2 * h + 1]));
-    grow |= top[h] > s.m[h] + kGrow;
+    // What stands behind them may be NaN in e4m3, and 0 * NaN must not reach the sums.
+    if (E4M3)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (2 * c + (t & 1) + (t >> 1) * 8 >= left)
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j) w[t][j] = 0;
   }
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[n][h] = fmaxf(z[n][h], z[n][2 + h]);
+      grow |= top[n][h] > s.m[n][h] + kGrow;
+    }
   if (__any_sync(0xffffffffu, grow)) {
-    const float unit = fmaxf(s.unit, f.vs);
+    const float unit = fmaxf(s.unit, fabsf(vs));
     const float ratio = unit > 0.f ? s.unit / unit : 0.f;
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float t = top[h];
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 1));
-      t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, 2));
-      t = fmaxf(t, s.m[h]);
-      const float corr = s.m[h] == -INFINITY ? 0.f : exp2_fast(s.m[h] - t);
-      s.m[h] = t;
-      s.l[h] *= corr;
+    for (int n = 0; n < N; ++n)
 #pragma unroll
-      for (int n = 0; n < DP / 8; ++n) {
-        s.o[n][2 * h] *= corr * ratio;
-        s.o[n][2 * h + 1] *= corr * ratio;
+      for (int h = 0; h < 2; ++h) {
+        float t = top[n][h];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+        t = fmaxf(t, s.m[n][h]);
+        const float corr = s.m[n][h] == -INFINITY ? 0.f : exp2_fast(s.m[n][h] - t);
+        s.m[n][h] = t;
+        s.l[n][h] *= corr;
+#pragma unroll
+        for (int t16 = 0; t16 < DP / 16; ++t16) {
+          s.o[n][t16][h] *= corr * ratio;
+          s.o[n][t16][2 + h] *= corr * ratio;
+        }
       }
-    }
     s.unit = unit;
     s.per = unit > 0.f ? 1.f / unit : 0.f;
   }
-  const float w = f.vs * s.per;
-  uint32_t p[2][H];
+  const float weight = vs * s.per;
+  uint32_t p[N][2];
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    const float m = s.m[h] == -INFINITY ? 0.f : s.m[h];
+  for (int n = 0; n < N; ++n) {
+    float e[4];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float m = s.m[n][h] == -INFINITY ? 0.f : s.m[n][h];
+      e[h] = exp2_fast(z[n][h] - m);
+      e[2 + h] = exp2_fast(z[n][2 + h] - m);
+      s.l[n][h] += e[h] + e[2 + h];
+    }
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      const float e0 = exp2_fast(z[t][2 * h] - m), e1 = exp2_fast(z[t][2 * h + 1] - m);
-      s.l[h] += e0 + e1;
-      const __half2 hv = __floats2half2_rn(e0 * w, e1 * w);
-      p[t][h] = *reinterpret_cast<const uint32_t*>(&hv);
+      const __half2 hv = __floats2half2_rn(e[2 * t] * weight, e[2 * t + 1] * weight);
+      p[n][t] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
     }
   }
-  const uint32_t a0 = p[0][0], a1 = H == 2 ? p[0][H - 1] : 0u, a2 = p[1][0],
-                 a3 = H == 2 ? p[1][H - 1] : 0u;
 #pragma unroll
   for (int j = 0; j < DP / 32; ++j) {
-    const uint32_t x01 = __byte_perm(f.v[0][j], f.v[1][j], 0x5140);
-    const uint32_t y01 = __byte_perm(f.v[0][j], f.v[1][j], 0x7362);
-    const uint32_t x23 = __byte_perm(f.v[2][j], f.v[3][j], 0x5140);
-    const uint32_t y23 = __byte_perm(f.v[2][j], f.v[3][j], 0x7362);
-    uint32_t b0, b1, b2, b3, c0, c1, c2, c3;
-    widen4<E4M3>(x01, b0, b1);
-    widen4<E4M3>(y01, b2, b3);
-    widen4<E4M3>(x23, c0, c1);
-    widen4<E4M3>(y23, c2, c3);
-    mma_16816(s.o[4 * j], a0, a1, a2, a3, b0, c0);
-    mma_16816(s.o[4 * j + 1], a0, a1, a2, a3, b1, c1);
-    mma_16816(s.o[4 * j + 2], a0, a1, a2, a3, b2, c2);
-    mma_16816(s.o[4 * j + 3], a0, a1, a2, a3, b3, c3);
+    uint32_t a[2][4];
+    {
+      const uint32_t x = __byte_perm(w[0][j], w[1][j], 0x5140), y = __byte_perm(w[0][j], w[1][j], 0x7362);
+      widen4<E4M3, false>(x, a[0][0], a[0][1]);
+      widen4<E4M3, false>(y, a[1][0], a[1][1]);
+    }
+    {
+      const uint32_t x = __byte_perm(w[2][j], w[3][j], 0x5140), y = __byte_perm(w[2][j], w[3][j], 0x7362);
+      widen4<E4M3, false>(x, a[0][2], a[0][3]);
+      widen4<E4M3, false>(y, a[1][2], a[1][3]);
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      mma_16816(s.o[n][2 * j], a[0], p[n][0], p[n][1]);
+      mma_16816(s.o[n][2 * j + 1], a[1], p[n][0], p[n][1]);
+    }
   }
 }
 
-template <int DP, int ROWS>
+template <int DP, int ROWS, bool E4M3>
 __device__ __forceinline__ void load_query(State<DP, ROWS>& s, const Args& a, int r, int head,
                                            int rg, int lane) {
-  constexpr int H = ROWS / 8;
+  constexpr int N = ROWS / 8;
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
-  for (int h = 0; h < H; ++h) {
-    const int row = rg * ROWS + 8 * h + g;
+  for (int n = 0; n < N; ++n) {
+    const int row = rg * ROWS + 8 * n + g;
     float x[DP / 4];
     float most = 0.f;
+    const int d0 = DP / 4 * c;           // this lane's dims
 #pragma unroll
-    for (int j = 0; j < DP / 64; ++j) {
-      const int d = 64 * j + 16 * c;
-      uint4 w[2] = {make_uint4(0, 0, 0, 0), make_uint4(0, 0, 0, 0)};
-      if (row < a.group && d < a.dim) {
-        const uint4* p = reinterpret_cast<const uint4*>(
-            static_cast<const uint16_t*>(a.q) + r * a.q_row +
-            static_cast<int64_t>(head * a.group + row) * a.q_head + d);
-        w[0] = __ldg(p);
-        w[1] = __ldg(p + 1);
-      }
-      const uint32_t u[8] = {w[0].x, w[0].y, w[0].z, w[0].w, w[1].x, w[1].y, w[1].z, w[1].w};
+    for (int j = 0; j < DP / 32; ++j) {
+      uint4 w = make_uint4(0, 0, 0, 0);
+      if (row < a.group && d0 + 8 * j < a.dim)
+        w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + r * a.q_row +
+                                                 static_cast<int64_t>(head * a.group + row) * a.q_head +
+                                                 d0 + 8 * j));
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
+      for (int i = 0; i < 4; ++i) {
         float2 v;
         if (a.bf16)
           v = make_float2(__uint_as_float(u[i] << 16), __uint_as_float(u[i] & 0xffff0000u));
         else
           v = __half22float2(*reinterpret_cast<const __half2*>(&u[i]));
-        x[16 * j + 2 * i] = v.x;
-        x[16 * j + 2 * i + 1] = v.y;
+        x[8 * j + 2 * i] = v.x;
+        x[8 * j + 2 * i + 1] = v.y;
         most = fmaxf(most, fmaxf(fabsf(v.x), fabsf(v.y)));
       }
     }
@@ -325,13 +328,24 @@ __device__ __forceinline__ void load_query(State<DP, ROWS>& s, const Args& a, in
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
     const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 126, -126), 126);
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    s.rf[h] = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    const float rf = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
       const __half2 lo = __floats2half2_rn(x[4 * i] * down, x[4 * i + 1] * down);
       const __half2 hi = __floats2half2_rn(x[4 * i + 2] * down, x[4 * i + 3] * down);
-      s.q[i][h] = *reinterpret_cast<const uint32_t*>(&lo);
-      s.q[i][H + h] = *reinterpret_cast<const uint32_t*>(&hi);
+      s.q[n][i][0] = *reinterpret_cast<const uint32_t*>(&lo);
+      s.q[n][i][1] = *reinterpret_cast<const uint32_t*>(&hi);
+      const float2 fl = __half22float2(lo), fh = __half22float2(hi);
+      sum += (fl.x + fl.y) + (fh.x + fh.y);
+    }
+    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s.rf[n][h] = __shfl_sync(0xffffffffu, rf, (2 * c + h) * 4);
+      const float t = __shfl_sync(0xffffffffu, sum, (2 * c + h) * 4);
+      s.start[n][h] = E4M3 ? 0.f : -kI8Offset * t;
     }
   }
 }
@@ -363,7 +377,7 @@ __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo,
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  for (int w = 0; w < kThreads / 32; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
@@ -371,23 +385,74 @@ __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo,
   return total;
 }
 
+// The segments of a CTA's range of tiles, in order: tiles t0 .. t1 of one
+// request and (virtual) head.
+struct Segments {
+  int64_t u, end;
+  int r, before;          // request, tiles before it
+  int heads;
+  int len, tiles, head, t0, t1;
+  __device__ __forceinline__ bool next(const Args& a) {
+    if (u >= end) return false;
+    while (true) {
+      len = length_of(a, r);
+      tiles = (len + kTile - 1) / kTile;
+      if (u < static_cast<int64_t>(before + tiles) * heads) break;
+      before += tiles;
+      ++r;
+    }
+    const int64_t in = u - static_cast<int64_t>(before) * heads;
+    head = static_cast<int>(in / tiles);
+    t0 = static_cast<int>(in % tiles);
+    t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - u)));
+    u += t1 - t0;
+    return true;
+  }
+};
+
+__device__ __forceinline__ void fail(int* err, volatile int* abort, int code) {
+  atomicCAS(err, 0, code);
+  *abort = 1;
+}
+
 template <int DP, int ROWS, bool E4M3>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(DP, ROWS)) cache_attention_kernel(const Args a) {
-  constexpr int H = ROWS / 8;
-  __shared__ float sm_o[kWarps][ROWS][DP];
-  __shared__ float sm_m[kWarps][ROWS], sm_l[kWarps][ROWS];
-  __shared__ int warp_sum[kWarps], start_r, start_p;
+__global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
+    cache_attention_kernel(const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const Args a) {
+  using L = Smem<DP, ROWS>;
+  constexpr int N = ROWS / 8;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  float2* scales = reinterpret_cast<float2*>(smem + L::kOffScales);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
+  uint64_t* empty = full + L::kStages;
+  int* misc = reinterpret_cast<int*>(smem + L::kOffMisc);
+  volatile int* abort_flag = misc;
+  int* warp_sum = misc + 1;              // [kThreads / 32]
+  int* start = misc + 8;                 // request, tiles before it
+  float* sm_m = reinterpret_cast<float*>(smem + L::kOffJoin);
+  float* sm_l = sm_m + kWarps * ROWS;
+  float* sm_o = reinterpret_cast<float*>(smem + L::kOffO);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int g = lane >> 2, c = lane & 3;
-  b2g::ptx::griddep_launch_dependents();
+  ptx::griddep_launch_dependents();
+  if (tid == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      ptx::mbar_init(&full[i], 1);
+      ptx::mbar_init(&empty[i], kWarps);
+    }
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+  }
 
   int lo, hi, run;
   const int total = scan_tiles(a, warp_sum, &lo, &hi, &run);
-  const int heads = a.kv_heads * a.row_groups;
-  const int64_t units = static_cast<int64_t>(total) * heads;
+  Segments seg;
+  seg.heads = a.kv_heads * a.row_groups;
+  const int64_t units = static_cast<int64_t>(total) * seg.heads;
   const int64_t share = (units + a.grid - 1) / a.grid;
-  int64_t u = blockIdx.x * share;
-  const int64_t end = min(u + share, units);
+  seg.u = blockIdx.x * share;
+  seg.end = min(seg.u + share, units);
   if (blockIdx.x == 0) {
     int p = run;
     for (int r = lo; r < hi; ++r) {
@@ -396,101 +461,162 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DP, ROWS)) cache_attenti
     }
     if (tid == 0) a.prefix[a.requests] = total;
   }
-  if (u >= end) return;
+  if (seg.u >= seg.end) return;
   {
     int p = run;
     for (int r = lo; r < hi; ++r) {
       const int t = tiles_of(a, r);
-      if (u >= static_cast<int64_t>(p) * heads && u < static_cast<int64_t>(p + t) * heads) {
-        start_r = r;
-        start_p = p;
+      if (seg.u >= static_cast<int64_t>(p) * seg.heads &&
+          seg.u < static_cast<int64_t>(p + t) * seg.heads) {
+        start[0] = r;
+        start[1] = p;
       }
       p += t;
     }
   }
   __syncthreads();
-  int r = start_r, p = start_p;
-  bool first = true;
-  while (u < end) {
-    const int len = length_of(a, r), tiles = (len + kTile - 1) / kTile;
-    const int64_t base = static_cast<int64_t>(p) * heads;
-    if (u >= base + static_cast<int64_t>(tiles) * heads) {
-      p += tiles;
-      ++r;
-      continue;
-    }
-    const int vh = static_cast<int>((u - base) / tiles);
-    const int t0 = static_cast<int>((u - base) % tiles);
-    const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - u)));
-    const int head = vh / a.row_groups, rg = vh % a.row_groups;
+  seg.r = start[0];
+  seg.before = start[1];
 
+  if (warp == kWarps) {
+    // ------------------------------------------------------------ producer
+    if (lane == 0) {
+      ptx::prefetch_tmap(&map_k);
+      ptx::prefetch_tmap(&map_v);
+    }
+    uint32_t n = 0;                      // stages filled
+    bool ok = true;
+    int had = -1;                        // request and first tile of the ids in `id`
+    int had_tile = 0, id = -1;
+    const int boxes = kTile / a.box_rows;        // of a stage
+    const int box_pieces = a.box_rows / 16;
+    const int box_bytes = a.box_rows * DP;
+    while (ok && seg.next(a)) {
+      const int32_t* row = a.table + seg.r * a.ld;
+      const int head = seg.head / a.row_groups;
+      float ks = 0.f, vs = 0.f;
+      for (int t = seg.t0; t < seg.t1 && ok; ++t) {
+        const int slot = n % L::kStages;
+        if (t == seg.t0 || t - had_tile >= 8) {
+          // Eight stages' blocks and scales at a time, one 16-token piece a lane.
+          if (had != seg.r || t < had_tile || t - had_tile >= 8) {
+            had = seg.r;
+            had_tile = t;
+            const int64_t token = static_cast<int64_t>(t) * kTile + 16 * lane;
+            id = token < seg.len ? __ldg(row + (token >> a.lg_block)) : -1;
+            if (static_cast<uint32_t>(id) >= a.num_blocks) id = -1;
+          }
+          ks = vs = 0.f;
+          if (id >= 0) {
+            ks = __ldg(a.k_scale + static_cast<int64_t>(id) * a.kv_heads + head);
+            vs = __ldg(a.v_scale + static_cast<int64_t>(id) * a.kv_heads + head);
+          }
+        }
+        if (!ptx::mbar_wait(&empty[slot], ((n / L::kStages) & 1) ^ 1, abort_flag, a.wait_limit_ns)) {
+          if (lane == 0) fail(a.err, abort_flag, kErrEmpty);
+          ok = false;
+          break;
+        }
+        const int first = (t - had_tile) * kWarps;       // lane of the stage's first piece
+        if (lane >= first && lane < first + kWarps)
+          // A block outside the cache leaves its tokens out.
+          scales[slot * kWarps + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
+        __syncwarp();
+        const int box_id = __shfl_sync(0xffffffffu, id, (first + lane * box_pieces) & 31);
+        const bool load = lane < boxes && box_id >= 0;
+        const unsigned loads = __ballot_sync(0xffffffffu, load);
+        if (lane == 0) ptx::mbar_arrive_expect_tx(&full[slot], __popc(loads) * 2 * box_bytes);
+        __syncwarp();
+        if (load) {
+          uint8_t* to = smem + slot * L::kStageBytes + lane * box_bytes;
+          const int off = (t * kTile + lane * a.box_rows) & ((1 << a.lg_block) - 1);
+          const int y = ((box_id * a.kv_heads + head) << a.lg_block) + off;
+          ptx::tma_load_2d(to, &map_k, &full[slot], 0, y);
+          ptx::tma_load_2d(to + L::kSideBytes, &map_v, &full[slot], 0, y);
+        }
+        __syncwarp();
+        ++n;
+      }
+    }
+    // Every load has landed before the CTA may leave (at once, but after a failure).
+    volatile int never = 0;
+    for (uint32_t e = n > L::kStages ? n - L::kStages : 0; e < n; ++e)
+      ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
+    return;
+  }
+
+  // -------------------------------------------------------------- consumers
+  const int g = lane >> 2, c = lane & 3;
+  uint32_t n = 0;
+  bool first = true;
+  while (seg.next(a)) {
+    const int head = seg.head / a.row_groups, rg = seg.head % a.row_groups;
     State<DP, ROWS> s;
 #pragma unroll
-    for (int h = 0; h < H; ++h) s.m[h] = -INFINITY, s.l[h] = 0.f;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) s.m[i][h] = -INFINITY, s.l[i][h] = 0.f;
     s.unit = s.per = 0.f;
 #pragma unroll
-    for (int n = 0; n < DP / 8; ++n)
+    for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int i = 0; i < 2 * H; ++i) s.o[n][i] = 0.f;
-
-    // This warp's tokens: 16 at t * kTile + warp * 16, t0 <= t < t1.
-    const int32_t* row = a.table + r * a.ld;
-    const int mask = (1 << a.lg_block) - 1;
-    const int w0 = warp * 16;
-    const int tend = min(t1, (len - w0 + kTile - 1) / kTile);   // tiles with tokens of this warp
-    auto block_at = [&](int t) { return t < tend ? __ldg(row + ((t * kTile + w0) >> a.lg_block)) : 0; };
-    Step<DP> f0, f1;
-    if (t0 < tend) {
-      int id = block_at(t0), next = block_at(t0 + 1);
-      load_step<DP>(f0, a, head, id, (t0 * kTile + w0) & mask, lane);
-      load_query<DP, ROWS>(s, a, r, head, rg, lane);
-      for (int t = t0; t < tend; t += 2) {
-        if (t + 1 < tend) load_step<DP>(f1, a, head, next, ((t + 1) * kTile + w0) & mask, lane);
-        next = block_at(t + 2);
-        compute_step<DP, ROWS, E4M3>(s, f0, len - t * kTile - w0, lane);
-        if (t + 1 >= tend) break;
-        if (t + 2 < tend) load_step<DP>(f0, a, head, next, ((t + 2) * kTile + w0) & mask, lane);
-        next = block_at(t + 3);
-        compute_step<DP, ROWS, E4M3>(s, f1, len - (t + 1) * kTile - w0, lane);
+      for (int t = 0; t < DP / 16; ++t) s.o[i][t][0] = s.o[i][t][1] = s.o[i][t][2] = s.o[i][t][3] = 0.f;
+    load_query<DP, ROWS, E4M3>(s, a, seg.r, head, rg, lane);
+    for (int t = seg.t0; t < seg.t1; ++t, ++n) {
+      const int slot = n % L::kStages;
+      if (!ptx::mbar_wait(&full[slot], (n / L::kStages) & 1, abort_flag, a.wait_limit_ns)) {
+        if (lane == 0) fail(a.err, abort_flag, kErrFull);
+        break;
       }
+      const int left = seg.len - t * kTile - warp * 16;
+      const float2 sc = scales[slot * kWarps + warp];
+      if (left > 0 && __float_as_uint(sc.x) != kNoBlock) {
+        const uint8_t* k = smem + slot * L::kStageBytes + warp * 16 * DP;
+        compute_piece<DP, ROWS, E4M3>(s, k, k + L::kSideBytes, sc.x, sc.y, left, lane);
+      }
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive(&empty[slot]);
     }
 
     // Join the four warps.
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      float l = s.l[h];
-      l += __shfl_xor_sync(0xffffffffu, l, 1);
-      l += __shfl_xor_sync(0xffffffffu, l, 2);
-      if (c == 0) {
-        sm_m[warp][8 * h + g] = s.m[h];
-        sm_l[warp][8 * h + g] = l;
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int y = warp * ROWS + 8 * i + 2 * c + h;
+        float l = s.l[i][h];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (g == 0) {
+          sm_m[y] = s.m[i][h];
+          sm_l[y] = l;
+        }
+#pragma unroll
+        for (int t = 0; t < DP / 16; t += 2)
+          *reinterpret_cast<float4*>(sm_o + y * DP + DP / 8 * g + 2 * t) =
+              make_float4(s.o[i][t][h] * s.unit, s.o[i][t][2 + h] * s.unit, s.o[i][t + 1][h] * s.unit,
+                          s.o[i][t + 1][2 + h] * s.unit);
       }
-#pragma unroll
-      for (int n = 0; n < 2; ++n)
-#pragma unroll
-        for (int i = 0; i < DP / 8; i += 4)
-          *reinterpret_cast<float4*>(&sm_o[warp][8 * h + g][DP / 8 * (2 * c + n) + i]) =
-              make_float4(s.o[i][2 * h + n] * s.unit, s.o[i + 1][2 * h + n] * s.unit,
-                          s.o[i + 2][2 * h + n] * s.unit, s.o[i + 3][2 * h + n] * s.unit);
-    }
-    __syncthreads();
-    const bool whole = t0 == 0 && t1 == tiles;
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
+    const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
     const int rows = min(ROWS, a.group - rg * ROWS);
-    for (int i = tid; i < rows * DP; i += kThreads) {
+    for (int i = tid; i < rows * DP; i += kWarps * 32) {
       const int y = i / DP, d = i % DP;
       float m = -INFINITY;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w][y]);
+      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w * ROWS + y]);
       float l = 0.f, o = 0.f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float e = sm_m[w][y] == -INFINITY ? 0.f : exp2_fast(sm_m[w][y] - m);
-        l += e * sm_l[w][y];
-        o += e * sm_o[w][y][d];
+        const float wm = sm_m[w * ROWS + y];
+        const float e = wm == -INFINITY ? 0.f : exp2_fast(wm - m);
+        l += e * sm_l[w * ROWS + y];
+        o += e * sm_o[(w * ROWS + y) * DP + d];
       }
       if (whole) {
-        const int64_t j = static_cast<int64_t>(r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
+        const int64_t j =
+            static_cast<int64_t>(seg.r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
         if (d < a.dim) store_out(a, j * a.dim + d, l > 0.f ? o / l : (l == 0.f ? 0.f : l));
         if (d == 0 && a.lse) a.lse[j] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       } else {
@@ -501,8 +627,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DP, ROWS)) cache_attenti
         }
       }
     }
-    __syncthreads();
-    u += t1 - t0;
+    asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
     first = false;
   }
 }
@@ -513,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(DP, ROWS)) cache_attenti
 template <int DP, int ROWS>
 __global__ void cache_join_kernel(const Args a) {
   extern __shared__ float sm[];          // [warps][DP + 1]
-  b2g::ptx::griddep_wait();
+  ptx::griddep_wait();
   const int heads = a.kv_heads * a.row_groups;
   const int j = blockIdx.x % (a.kv_heads * a.group), r = blockIdx.x / (a.kv_heads * a.group);
   const int head = j / a.group, row = j % a.group, rg = row / ROWS, y = row % ROWS;
@@ -575,7 +700,7 @@ int check(const b2g_cache_attention_desc* d) {
   if (d->block_size < 16 || d->block_size > 256 || (d->block_size & (d->block_size - 1)) ||
       d->dim % 16 || d->dim > 128 || d->num_blocks > 0x7fffffff ||
       d->table_width * d->block_size > 0x7fffffc0 || d->requests > (1 << 20) ||
-      d->heads > (1 << 16) || d->requests * d->heads > 0x7fffffff)
+      d->num_blocks * d->kv_heads * d->block_size > 0x7fffffff || d->heads > (1 << 16) || d->requests * d->heads > 0x7fffffff)
     return B2G_ERR_UNSUPPORTED;
   return B2G_OK;
 }
@@ -594,7 +719,7 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   const int64_t most = d->requests * d->kv_heads * w.row_groups *
                        std::max<int64_t>(cdiv(d->table_width * d->block_size, kTile), 1);
   w.grid = static_cast<int>(std::min<int64_t>(
-      std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * ctas_per_sm(w.dp, w.rows)));
+      std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * (w.rows == 8 ? Smem<128, 8>::kCtas : Smem<128, 16>::kCtas)));
   auto pad = [](int64_t n) { return cdiv(n, 256) * 256; };
   w.off_m = pad((d->requests + 1) * 4);
   w.off_l = w.off_m + pad(2ll * w.grid * w.rows * 4);
@@ -603,9 +728,30 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   return w;
 }
 
+// The codes of a cache as rows of dim bytes; a box is box_rows rows of DP
+// bytes (zeros past dim) in the swizzle of that width.
+bool make_map(CUtensorMap* map, const void* base, int64_t dim, int64_t rows, int dp, int box_rows) {
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(dim)};
+  const cuuint32_t box[2] = {static_cast<cuuint32_t>(dp), static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  return b2g::encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, base, dims, strides, box, estr,
+                           dp == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
 template <int DP, int ROWS, bool E4M3>
-int launch(const Args& a, cudaStream_t stream) {
-  cache_attention_kernel<DP, ROWS, E4M3><<<a.grid, kThreads, 0, stream>>>(a);
+int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStream_t stream) {
+  using L = Smem<DP, ROWS>;
+  static thread_local int configured = -1;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (configured != dev) {
+    if (cudaFuncSetAttribute(cache_attention_kernel<DP, ROWS, E4M3>,
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes) != cudaSuccess)
+      return B2G_ERR_LAUNCH;
+    configured = dev;
+  }
+  cache_attention_kernel<DP, ROWS, E4M3><<<a.grid, kThreads, L::kBytes, stream>>>(mk, mv, a);
   if (cudaGetLastError() != cudaSuccess) return B2G_ERR_LAUNCH;
   const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
   // Parts of a head, were all lengths alike.
@@ -653,8 +799,6 @@ extern "C" int b2g_cache_attention(const b2g_cache_attention_desc* d, b2g_stream
   a.q = d->q;
   a.q_row = d->q_row_stride;
   a.q_head = d->q_head_stride;
-  a.k_cache = static_cast<const uint8_t*>(d->k_cache);
-  a.v_cache = static_cast<const uint8_t*>(d->v_cache);
   a.k_scale = d->k_scale;
   a.v_scale = d->v_scale;
   a.table = d->block_table;
@@ -681,11 +825,19 @@ extern "C" int b2g_cache_attention(const b2g_cache_attention_desc* d, b2g_stream
   a.part_l = reinterpret_cast<float*>(ws + w.off_l);
   a.part_o = reinterpret_cast<float*>(ws + w.off_o);
   a.grid = w.grid;
+  a.wait_limit_ns = b2g::current_wait_limit_ns();
+  a.err = dev.error_word;
+  a.box_rows = static_cast<int>(std::min<int64_t>(d->block_size, kTile));
+  CUtensorMap mk = {}, mv = {};
+  const int64_t cache_rows = d->num_blocks * d->kv_heads * d->block_size;
+  if (d->num_blocks > 0 && (!make_map(&mk, d->k_cache, d->dim, cache_rows, w.dp, a.box_rows) ||
+                            !make_map(&mv, d->v_cache, d->dim, cache_rows, w.dp, a.box_rows)))
+    return B2G_ERR_UNSUPPORTED;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool e4 = d->codes == B2G_E4M3;
   if (w.dp == 64)
-    return w.rows == 8 ? (e4 ? launch<64, 8, true>(a, stream) : launch<64, 8, false>(a, stream))
-                       : (e4 ? launch<64, 16, true>(a, stream) : launch<64, 16, false>(a, stream));
-  return w.rows == 8 ? (e4 ? launch<128, 8, true>(a, stream) : launch<128, 8, false>(a, stream))
-                     : (e4 ? launch<128, 16, true>(a, stream) : launch<128, 16, false>(a, stream));
+    return w.rows == 8 ? (e4 ? launch<64, 8, true>(mk, mv, a, stream) : launch<64, 8, false>(mk, mv, a, stream))
+                       : (e4 ? launch<64, 16, true>(mk, mv, a, stream) : launch<64, 16, false>(mk, mv, a, stream));
+  return w.rows == 8 ? (e4 ? launch<128, 8, true>(mk, mv, a, stream) : launch<128, 8, false>(mk, mv, a, stream))
+                     : (e4 ? launch<128, 16, true>(mk, mv, a, stream) : launch<128, 16, false>(mk, mv, a, stream));
 }

@@ -804,6 +804,14 @@ int current_device(Device* out) {
   if (rc == B2G_OK) *out = Device{ds->num_sms, ds->err_word};
   return rc;
 }
+bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                  const cuuint32_t* element_strides, CUtensorMapSwizzle swizzle) {
+  EncodeTiledFn fn = encode_fn();
+  return fn && fn(map, type, rank, const_cast<void*>(base), dims, strides, box, element_strides,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
 long long current_wait_limit_ns() { return wait_limit_ns(); }
 bool pdl_enabled() { return B2G_PDL != 0; }
 }  // namespace b2g

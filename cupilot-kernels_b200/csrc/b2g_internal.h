@@ -2,6 +2,8 @@
 // (not part of the C ABI; hidden symbols).
 #pragma once
 
+#include <cuda.h>
+
 namespace b2g {
 
 // Device address of the current device's error word (the one
@@ -16,6 +18,13 @@ struct Device {
   int* error_word = nullptr;
 };
 int current_device(Device* out);
+
+// cuTensorMapEncodeTiled (through the runtime's entry point), without
+// interleave, 256-byte L2 promotion, zeros outside.  false: not to be had, or
+// the driver refuses the layout.
+bool encode_tiled(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box,
+                  const cuuint32_t* element_strides, CUtensorMapSwizzle swizzle);
 
 // Bound on every device-side wait, in ns (B2G_WAIT_LIMIT_MS, default 2 s).
 long long current_wait_limit_ns();

@@ -25,7 +25,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstdint>
-#include <mutex>
 
 #include "../../include/b2g_serving.h"
 #include "b2g_internal.h"
@@ -481,30 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*,
-                                   const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                   CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(ptr);
-  });
-  return fn;
-}
-
 // {dim, heads, tokens} in 16 bits; a box is 64 columns of box_heads heads of
 // box_tokens tokens, rows of 128 bytes in the 128-byte swizzle.
 bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_t heads, int64_t tokens,
               int64_t head_stride, int64_t token_stride, int box_heads, int box_tokens) {
-  EncodeTiledFn fn = encode_fn();
-  if (!fn) return false;
   if (heads == 1) head_stride = dim;
   if (tokens == 1) token_stride = std::max<int64_t>(heads * dim, head_stride);
   cuuint64_t dims[3] = {static_cast<cuuint64_t>(dim), static_cast<cuuint64_t>(heads),
@@ -513,10 +492,8 @@ bool make_map(CUtensorMap* map, const void* base, bool bf16, int64_t dim, int64_
                            static_cast<cuuint64_t>(token_stride) * 2};
   cuuint32_t box[3] = {64, static_cast<cuuint32_t>(box_heads), static_cast<cuuint32_t>(box_tokens)};
   cuuint32_t estr[3] = {1, 1, 1};
-  return fn(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
-            const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+  return encode_tiled(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                      3, base, dims, strides, box, estr, CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int DP, bool BF16>
