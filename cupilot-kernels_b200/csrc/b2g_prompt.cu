@@ -7,17 +7,23 @@
 //   O = O exp(m - m') + P V.
 // The rows of a tile are tokens times the query heads that share a kv head
 // (row = token * group + head, one TMA box), so K and V are read once for the
-// group and a group's short prompt still fills a tile.  A CTA takes two such
-// tiles of one sequence and kv head.  S, P and O live in tensor memory: S0 S1
-// O0 O1, 128 columns each, P over the first half of its S.
+// group and a group's short prompt still fills a tile.  A work item is two
+// such tiles of one sequence and kv head; a CTA does one after another, the
+// later ones taken over from CTAs that have not started.  S, P and O live in
+// tensor memory: S0 S1 O0 O1, 128 columns each, P over the first half of its
+// S.
 //   warps 0-3, 4-7   softmax of tile 0 / 1, a thread a row: S from tensor
 //                    memory, P back in 16 bits, at the end O / l to memory
 //   warp 8           the products: while one tile's softmax runs, the other
 //                    tile's P V and next Q K^T keep the tensor cores busy
 //   warp 9           TMA loads: Q, then K and V tiles through a ring
+//   warp 10          the next work item
 // The maximum is taken over only where it grew by more than 2^8 (P stays
 // within 16 bits' range, l and O are fp32): then, rarely, the softmax warps
 // rescale O themselves.
+// Bound by the exponentials beside the products: a pair of tiles has 2^15 of
+// them against 2048 cycles of tensor core work (dim 128), and the special
+// function unit gives 16 a cycle; part of them is computed on the FMA units.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -36,13 +42,20 @@ namespace prompt {
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr int kSoftmaxWarps = 8;
-constexpr int kThreads = (kSoftmaxWarps + 2) * 32;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kNextWarp = 10;
+constexpr int kThreads = 12 * 32;     // a whole third warpgroup, for the register split
+// Registers: 384 threads start with 168 each; the third warpgroup gives 96 of
+// each thread's to the softmax warps (2 * 128 * 216 + 128 * 72 = 384 * 168).
+constexpr int kRegsSoftmax = 216, kRegsOther = 72;
+constexpr int kItemReaders = kSoftmaxWarps + 2;
+// Of 16 pairs of exponentials, how many run on the FMA units.
+constexpr int kPolyPairs = 5;
 constexpr float kGrow = 8.f;
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kBoxBytes = 128 * 128;  // 64 columns x 128 rows of 16 bits
 
 enum : int { kErrFull = 0x301, kErrEmpty = 0x302, kErrS = 0x303, kErrP = 0x304, kErrO = 0x305,
-             kErrQ = 0x306 };
+             kErrQ = 0x306, kErrItem = 0x307, kErrNext = 0x308 };
 
 template <int DP>
 struct Smem {
@@ -51,9 +64,11 @@ struct Smem {
   static constexpr int kStages = DP == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;
   static constexpr int kOffBars = kOffRing + kStages * kTileBytes;
-  static constexpr int kNumBars = 2 * kStages + 2 * 4 + 1;
-  static constexpr int kOffMisc = kOffBars + kNumBars * 8;
-  static constexpr int kBytes = kOffMisc + 64 + 1024;
+  static constexpr int kNumBars = 2 * kStages + 2 * 5 + 4 + 2;
+  static constexpr int kOffNext = (kOffBars + kNumBars * 8 + 15) / 16 * 16;   // 16-byte answer
+  static constexpr int kOffItems = kOffNext + 16;
+  static constexpr int kOffMisc = kOffItems + 2 * 48;
+  static constexpr int kBytes = kOffMisc + 16 + 1024;
 };
 static_assert(Smem<128>::kBytes <= 232448 && Smem<64>::kBytes <= 232448, "shared memory budget");
 
@@ -106,6 +121,14 @@ __device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[
       "r"(r[29]), "r"(r[30]), "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void tmem_st_wait() {
   asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 }
@@ -125,13 +148,85 @@ __device__ __forceinline__ uint32_t pack(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// What a CTA works on; all lengths cut to the tensors' sizes.
+// Pairs of fp32 in one register pair.
+__device__ __forceinline__ uint64_t pair(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpair(uint64_t r, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(r));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+// Maxima that keep a NaN.
+__device__ __forceinline__ float max2(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// 2^x of a pair by range reduction and a polynomial: x = n + f, |f| <= 1/2,
+// 2^f by its best relative approximation of degree 3 (error 7.5e-5, for P in
+// bf16 with its rounding of 2e-3) or 4 (2.6e-6, for fp16 with 2.4e-4), the
+// coefficients found by Remez exchange; n goes into the exponent.  Below
+// 2^-126 it stays there, which is nothing beside the row's maximum.
+template <bool BF16>
+__device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
+  float x, y;
+  unpair(x2, x, y);
+  x2 = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  const float big = 12582912.f;                     // 1.5 * 2^23: the sum's low bits are n
+  const uint64_t n2 = add2(x2, pair(big, big));
+  const uint64_t back = add2(n2, pair(-big, -big));
+  const uint64_t f2 = fma2(back, pair(-1.f, -1.f), x2);
+  uint64_t y2;
+  if (BF16) {
+    y2 = fma2(f2, pair(0.05517167f, 0.05517167f), pair(0.24261113f, 0.24261113f));
+    y2 = fma2(f2, y2, pair(0.69326097f, 0.69326097f));
+    y2 = fma2(f2, y2, pair(0.99992806f, 0.99992806f));
+  } else {
+    y2 = fma2(f2, pair(0.009570102f, 0.009570102f), pair(0.05591786f, 0.05591786f));
+    y2 = fma2(f2, y2, pair(0.24024744f, 0.24024744f));
+    y2 = fma2(f2, y2, pair(0.6931218f, 0.6931218f));
+    y2 = fma2(f2, y2, pair(0.9999993f, 0.9999993f));
+  }
+  float na, nb;
+  unpair(n2, na, nb);
+  unpair(y2, a, b);
+  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
+  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+}
+
+// Two tiles of one sequence and kv head; all lengths cut to the tensors' sizes.
 struct Item {
   int q0, qlen, k0, klen, first;      // first: token of tile 0's row 0, within the sequence
   int head;
+  int n0, n1;                         // key tiles of each row tile (0: no rows, or they see nothing)
+  int more;                           // 0: no work is left
 };
+static_assert(sizeof(Item) <= 48, "item slot");
 
 __device__ __forceinline__ int clampi(int v, int lo, int hi) { return min(max(v, lo), hi); }
+
+// Keys that token `tok` of the sequence sees.
+__device__ __forceinline__ int keys_of(const Params& p, const Item& it, int tok) {
+  if (!p.causal) return it.klen;
+  return clampi(tok + it.klen - it.qlen + 1, 0, it.klen);
+}
 
 // Tile pair x of all sequences: sequence s owns the places from
 // cu[s] / span + s on, at least as many as it has pairs; some stay empty.
@@ -149,13 +244,31 @@ __device__ __forceinline__ bool find_item(const Params& p, int x, int head, Item
   it->k0 = clampi(p.cu_k[lo], 0, p.tokens_k);
   it->klen = max(clampi(p.cu_k[lo + 1], 0, p.tokens_k) - it->k0, 0);
   it->first = (x - it->q0 / span - lo) * span;
+  auto tiles = [&](int t0) {
+    const int last = min(t0 + p.tile_tokens, it->qlen) - 1;
+    return t0 < it->qlen ? (keys_of(p, *it, last) + kKeys - 1) / kKeys : 0;
+  };
+  it->n0 = tiles(it->first);
+  it->n1 = tiles(it->first + p.tile_tokens);
   return it->first >= 0 && it->first < it->qlen;
 }
 
-// Keys that token `tok` of the sequence sees.
-__device__ __forceinline__ int keys_of(const Params& p, const Item& it, int tok) {
-  if (!p.causal) return it.klen;
-  return clampi(tok + it.klen - it.qlen + 1, 0, it.klen);
+// Rows of no sequence: zeros, a share for each of the first work indices.
+__device__ __forceinline__ void zero_rows(const Params& p, int w, int lane) {
+  constexpr int kShares = 64;
+  const int shares = min(kShares, p.slots * p.kv_heads);
+  if (w >= shares) return;
+  const int before = p.sequences ? clampi(p.cu_q[0], 0, p.tokens) : 0;
+  const int after = p.sequences ? clampi(p.cu_q[p.sequences], before, p.tokens) : 0;
+  const int64_t n = static_cast<int64_t>(before + p.tokens - after) * p.heads;
+  for (int64_t i = static_cast<int64_t>(w) * 32 + lane; i < n; i += shares * 32) {
+    int64_t t = i / p.heads;
+    const int h = static_cast<int>(i % p.heads);
+    if (t >= before) t += after - before;
+    uint16_t* o = p.out + t * p.out_token + h * p.out_head;
+    for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
+    if (p.lse) p.lse[t * p.heads + h] = -INFINITY;
+  }
 }
 
 template <int DP, bool BF16>
@@ -169,54 +282,40 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kOffBars);
   uint64_t* empty = full + L::kStages;
   uint64_t* q_full = empty + L::kStages;     // [2]
-  uint64_t* s_full = q_full + 2;             // [2] S of the tile is complete
-  uint64_t* p_ready = q_full + 4;            // [2] P of the tile is stored
-  uint64_t* o_done = q_full + 6;             // [2] P V of the tile is added to O
-  uint64_t* drain = q_full + 8;
+  uint64_t* q_empty = q_full + 2;            // [2] the tile's last Q K^T has read Q
+  uint64_t* s_full = q_full + 4;             // [2] S of the tile is complete
+  uint64_t* p_ready = q_full + 6;            // [2] P of the tile is stored
+  uint64_t* o_done = q_full + 8;             // [2] P V of the tile is added to O
+  uint64_t* item_full = q_full + 10;         // [2]
+  uint64_t* item_empty = q_full + 12;        // [2]
+  uint64_t* next_full = q_full + 14;
+  uint64_t* drain = q_full + 15;
+  uint8_t* next_answer = smem + L::kOffNext;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
-  int* has_item = reinterpret_cast<int*>(smem + L::kOffMisc + 8);
-  Item* item = reinterpret_cast<Item*>(smem + L::kOffMisc + 16);
+  auto item_at = [&](uint32_t k) { return reinterpret_cast<Item*>(smem + L::kOffItems + (k & 1) * 48); };
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-
-  // Rows of no sequence.
-  {
-    const int before = p.sequences ? clampi(p.cu_q[0], 0, p.tokens) : 0;
-    const int after = p.sequences ? clampi(p.cu_q[p.sequences], 0, p.tokens) : 0;
-    const int64_t n = static_cast<int64_t>(before + p.tokens - after) * p.heads;
-    for (int64_t i = static_cast<int64_t>(blockIdx.x) * kThreads + tid; i < n;
-         i += static_cast<int64_t>(gridDim.x) * kThreads) {
-      int64_t t = i / p.heads;
-      const int h = static_cast<int>(i % p.heads);
-      if (t >= before) t += after - before;
-      uint16_t* o = p.out + t * p.out_token + h * p.out_head;
-      for (int d = 0; d < p.dim; d += 8) *reinterpret_cast<uint4*>(o + d) = make_uint4(0, 0, 0, 0);
-      if (p.lse) p.lse[t * p.heads + h] = -INFINITY;
-    }
-  }
   if (tid == 0) {
-    // Late tiles see the most keys: they go first.
-    *has_item = p.sequences > 0 && find_item(p, p.slots - 1 - static_cast<int>(blockIdx.x) / p.kv_heads,
-                                             static_cast<int>(blockIdx.x) % p.kv_heads, item);
     for (int s = 0; s < L::kStages; ++s) {
       ptx::mbar_init(&full[s], 1);
       ptx::mbar_init(&empty[s], 1);
     }
     for (int i = 0; i < 2; ++i) {
       ptx::mbar_init(&q_full[i], 1);
+      ptx::mbar_init(&q_empty[i], 1);
       ptx::mbar_init(&s_full[i], 1);
       ptx::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
       ptx::mbar_init(&o_done[i], 1);
+      ptx::mbar_init(&item_full[i], 1);
+      ptx::mbar_init(&item_empty[i], kItemReaders);
     }
+    ptx::mbar_init(next_full, 1);
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
   }
-  __syncthreads();
-  if (!*has_item) return;
-  const Item it = *item;
-  if (warp == kSoftmaxWarps) {
+  if (warp == kMmaWarp) {
     ptx::tmem_alloc(tmem_slot, 512);
     ptx::tmem_relinquish();
   }
@@ -225,227 +324,337 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  // Key tiles of each row tile (none: the tile has no rows, or they see nothing).
-  int n_of[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int t0 = it.first + i * p.tile_tokens;
-    const int last = min(t0 + p.tile_tokens, it.qlen) - 1;
-    n_of[i] = t0 < it.qlen ? (keys_of(p, it, last) + kKeys - 1) / kKeys : 0;
-  }
-  const int n0 = n_of[0], n1 = n_of[1], n = max(n0, n1);
+  // The k-th item of this CTA, for the warps that work on it.
+  auto get_item = [&](uint32_t k, Item* it) {
+    if (!ptx::mbar_wait(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns)) {
+      if (lane == 0) fail(p.err, abort_flag, kErrItem);
+      return false;
+    }
+    *it = *item_at(k);
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive(&item_empty[k & 1]);
+    return it->more != 0;
+  };
 
-  if (warp == kSoftmaxWarps + 1) {
-    // ------------------------------------------------------------ loads
-    if (lane == 0 && n > 0) {
-      ptx::prefetch_tmap(&map_q);
-      ptx::prefetch_tmap(&map_k);
-      ptx::prefetch_tmap(&map_v);
-      const uint32_t q_bytes = L::kBoxes * p.group * p.tile_tokens * 128;
-      auto load_q = [&](int i) {
-        ptx::mbar_arrive_expect_tx(&q_full[i], q_bytes);
-        for (int b = 0; b < L::kBoxes; ++b)
-          ptx::tma_load_3d(smem + i * L::kTileBytes + b * kBoxBytes, &map_q, &q_full[i], b * 64,
-                           it.head * p.group, it.q0 + it.first + i * p.tile_tokens);
-      };
-      int issued = 0;
-      bool ok = true;
-      auto load_kv = [&](const CUtensorMap* map, int j) {
-        const int s = issued % L::kStages;
-        if (!ptx::mbar_wait(&empty[s], ((issued / L::kStages) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
-          fail(p.err, abort_flag, kErrEmpty);
-          return false;
+  if (warp >= kSoftmaxWarps) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsOther));
+    if (warp == kNextWarp) {
+      // ---------------------------------------------------------- next item
+      int w = blockIdx.x;
+      uint32_t k = 0, asked = 0;
+      bool more = true;
+      while (more) {
+        // Ask for another CTA's work now, use it when this item is handed out.
+        if (lane == 0) {
+          ptx::fence_proxy_async_smem();
+          ptx::mbar_arrive_expect_tx(next_full, 16);
+          ptx::clc_try_cancel(next_answer, next_full);
         }
-        ptx::mbar_arrive_expect_tx(&full[s], L::kTileBytes);
-        for (int b = 0; b < L::kBoxes; ++b)
-          ptx::tma_load_3d(smem + L::kOffRing + s * L::kTileBytes + b * kBoxBytes, map, &full[s],
-                           b * 64, it.head, it.k0 + j * kKeys);
-        ++issued;
-        return true;
-      };
-      load_q(0);
-      ok = load_kv(&map_k, 0);
-      load_q(1);
-      ok = ok && load_kv(&map_v, 0);
-      for (int j = 1; j < n && ok; ++j) ok = load_kv(&map_k, j) && load_kv(&map_v, j);
-      // Every load has landed before the CTA may leave.
-      volatile int never = 0;
-      for (int i = 0; i < 2; ++i) ptx::mbar_wait(&q_full[i], 0, &never, kDrainLimitNs);
-      for (int e = max(0, issued - L::kStages); e < issued; ++e)
-        ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
-    }
-  } else if (warp == kSoftmaxWarps) {
-    // ------------------------------------------------------------ products
-    constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
-    const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
-    const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
-    const uint32_t ring = ptx::smem_addr(smem + L::kOffRing);
-    bool ok = n > 0;
-    auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-      if (!ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) {
-        if (lane == 0) fail(p.err, abort_flag, code);
-        return false;
-      }
-      ptx::tc_fence_after();
-      return true;
-    };
-    auto wait_full = [&](int e) {
-      return wait(&full[e % L::kStages], (e / L::kStages) & 1, kErrFull);
-    };
-    auto scores = [&](int i, int e) {      // S_i = Q_i K^T, K in ring entry e
-      const uint32_t sq = ptx::smem_addr(smem + i * L::kTileBytes);
-      const uint32_t sk = ring + (e % L::kStages) * L::kTileBytes;
-      for (int k = 0; k < p.dim / 16; ++k) {
-        const uint32_t at = (k >> 2) * kBoxBytes + (k & 3) * 32;
-        ptx::mma_f16(tmem + i * kKeys, ptx::smem_desc(sq + at, 16, 1024, ptx::kLayoutSw128),
-                     ptx::smem_desc(sk + at, 16, 1024, ptx::kLayoutSw128), idesc_s, k > 0);
-      }
-      ptx::mma_commit(&s_full[i]);
-    };
-    auto values = [&](int i, int e, bool add) {   // O_i += P_i V, V in ring entry e
-      const uint32_t sv = ring + (e % L::kStages) * L::kTileBytes;
-      for (int k = 0; k < kKeys / 16; ++k)
-        mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8,
-               ptx::smem_desc(sv + k * 16 * 128, kBoxBytes, 1024, ptx::kLayoutSw128), idesc_o,
-               add || k > 0);
-      ptx::mma_commit(&o_done[i]);
-    };
-    if (ok) ok = wait(&q_full[0], 0, kErrQ) && wait(&q_full[1], 0, kErrQ) && wait_full(0);
-    if (ok && lane == 0) {
-      if (n0 > 0) scores(0, 0);
-      if (n1 > 0) scores(1, 0);
-      ptx::mma_commit(&empty[0]);
-    }
-    for (int j = 0; j < n && ok; ++j) {
-      const int ek = 2 * (j + 1), ev = 2 * j + 1;
-      ok = wait_full(ev);
-      if (!ok) break;
-      if ((j + 1) * kKeys > it.klen) {
-        // Rows past the sequence hold the next one's values (or nothing): their weights are 0,
-        // but 0 * inf is not.
-        uint8_t* v = smem + L::kOffRing + (ev % L::kStages) * L::kTileBytes;
-        const int from = (it.klen - j * kKeys) * 128;
-        for (int b = 0; b < L::kBoxes; ++b)
-          for (int x = from + lane * 16; x < kBoxBytes; x += 512)
-            *reinterpret_cast<uint4*>(v + b * kBoxBytes + x) = make_uint4(0, 0, 0, 0);
-        ptx::fence_proxy_async_smem();
+        zero_rows(p, w, lane);
+        Item it;
+        // Late tiles see the most keys: they go first.
+        bool work = p.sequences > 0 && find_item(p, p.slots - 1 - w / p.kv_heads, w % p.kv_heads, &it);
+        if (work) {
+          if (!ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+            if (lane == 0) fail(p.err, abort_flag, kErrItem);
+            more = false;
+          } else {
+            it.more = 1;
+            if (lane == 0) {
+              *item_at(k) = it;
+              ptx::mbar_arrive(&item_full[k & 1]);
+            }
+            ++k;
+          }
+        }
+        // (waited for even after a failure: the answer has to land before the CTA leaves)
+        volatile int never = 0;
+        if (!ptx::mbar_wait(next_full, asked & 1, &never, p.wait_limit_ns)) {
+          if (lane == 0) fail(p.err, abort_flag, kErrNext);
+          more = false;
+        } else if (!ptx::clc_answer(next_answer, &w)) {
+          more = false;
+        }
+        ++asked;
         __syncwarp();
       }
-      if (j + 1 < n) ok = wait_full(ek);
-      for (int i = 0; i < 2 && ok; ++i) {
-        const int ni = i ? n1 : n0;
-        if (j < ni) {
-          ok = wait(&p_ready[i], j & 1, kErrP);
-          if (ok && lane == 0) values(i, ev, j > 0);
+      if (ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+        if (lane == 0) {
+          item_at(k)->more = 0;
+          ptx::mbar_arrive(&item_full[k & 1]);
         }
-        if (ok && j + 1 < ni && lane == 0) scores(i, ek);
       }
+      __syncwarp();
+    } else if (warp == kLoadWarp) {
+      // ---------------------------------------------------------- loads
       if (lane == 0) {
-        ptx::mma_commit(&empty[ev % L::kStages]);
-        if (j + 1 < n) ptx::mma_commit(&empty[ek % L::kStages]);
+        ptx::prefetch_tmap(&map_q);
+        ptx::prefetch_tmap(&map_k);
+        ptx::prefetch_tmap(&map_v);
+      }
+      const uint32_t q_bytes = L::kBoxes * p.group * p.tile_tokens * 128;
+      uint32_t q_issued[2] = {0, 0}, issued = 0;
+      bool ok = true;
+      Item it;
+      for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
+        if (lane == 0) {
+          auto load_q = [&](int i) {
+            if (!ptx::mbar_wait(&q_empty[i], (q_issued[i] & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+              fail(p.err, abort_flag, kErrEmpty);
+              return false;
+            }
+            ptx::mbar_arrive_expect_tx(&q_full[i], q_bytes);
+            for (int b = 0; b < L::kBoxes; ++b)
+              ptx::tma_load_3d(smem + i * L::kTileBytes + b * kBoxBytes, &map_q, &q_full[i], b * 64,
+                               it.head * p.group, it.q0 + it.first + i * p.tile_tokens);
+            ++q_issued[i];
+            return true;
+          };
+          auto load_kv = [&](const CUtensorMap* map, int j) {
+            const uint32_t s = issued % L::kStages;
+            if (!ptx::mbar_wait(&empty[s], ((issued / L::kStages) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+              fail(p.err, abort_flag, kErrEmpty);
+              return false;
+            }
+            ptx::mbar_arrive_expect_tx(&full[s], L::kTileBytes);
+            for (int b = 0; b < L::kBoxes; ++b)
+              ptx::tma_load_3d(smem + L::kOffRing + s * L::kTileBytes + b * kBoxBytes, map, &full[s],
+                               b * 64, it.head, it.k0 + j * kKeys);
+            ++issued;
+            return true;
+          };
+          const int n = max(it.n0, it.n1);
+          if (it.n0 > 0) ok = load_q(0);
+          if (n > 0) ok = ok && load_kv(&map_k, 0);
+          if (it.n1 > 0) ok = ok && load_q(1);
+          if (n > 0) ok = ok && load_kv(&map_v, 0);
+          for (int j = 1; j < n && ok; ++j) ok = load_kv(&map_k, j) && load_kv(&map_v, j);
+        }
+        ok = __shfl_sync(0xffffffffu, ok, 0);
+      }
+      // Every load has landed before the CTA may leave.
+      if (lane == 0) {
+        volatile int never = 0;
+        for (int i = 0; i < 2; ++i)
+          if (q_issued[i]) ptx::mbar_wait(&q_full[i], (q_issued[i] - 1) & 1, &never, kDrainLimitNs);
+        for (uint32_t e = issued > L::kStages ? issued - L::kStages : 0; e < issued; ++e)
+          ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
+      }
+      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------- products
+      constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+      const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
+      const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
+      const uint32_t ring = ptx::smem_addr(smem + L::kOffRing);
+      uint32_t q_used[2] = {0, 0}, steps[2] = {0, 0}, used = 0;
+      bool ok = true;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+        if (!ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) {
+          if (lane == 0) fail(p.err, abort_flag, code);
+          return false;
+        }
+        ptx::tc_fence_after();
+        return true;
+      };
+      auto wait_full = [&](uint32_t e) {
+        return wait(&full[e % L::kStages], (e / L::kStages) & 1, kErrFull);
+      };
+      auto scores = [&](int i, uint32_t e, bool last) {      // S_i = Q_i K^T, K in ring entry e
+        const uint32_t sq = ptx::smem_addr(smem + i * L::kTileBytes);
+        const uint32_t sk = ring + (e % L::kStages) * L::kTileBytes;
+        for (int k = 0; k < p.dim / 16; ++k) {
+          const uint32_t at = (k >> 2) * kBoxBytes + (k & 3) * 32;
+          ptx::mma_f16(tmem + i * kKeys, ptx::smem_desc(sq + at, 16, 1024, ptx::kLayoutSw128),
+                       ptx::smem_desc(sk + at, 16, 1024, ptx::kLayoutSw128), idesc_s, k > 0);
+        }
+        ptx::mma_commit(&s_full[i]);
+        if (last) ptx::mma_commit(&q_empty[i]);
+      };
+      auto values = [&](int i, uint32_t e, bool add) {   // O_i += P_i V, V in ring entry e
+        const uint32_t sv = ring + (e % L::kStages) * L::kTileBytes;
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)
+          mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8,
+                 ptx::smem_desc(sv + k * 16 * 128, kBoxBytes, 1024, ptx::kLayoutSw128), idesc_o,
+                 add || k > 0);
+        ptx::mma_commit(&o_done[i]);
+      };
+      Item it;
+      for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
+        const int n = max(it.n0, it.n1);
+        if (n == 0) continue;
+        ok = wait_full(used);
+        for (int i = 0; i < 2 && ok; ++i) {
+          const int ni = i ? it.n1 : it.n0;
+          if (ni == 0) continue;
+          ok = wait(&q_full[i], q_used[i]++ & 1, kErrQ);
+          if (ok && lane == 0) scores(i, used, ni == 1);
+        }
+        if (lane == 0) ptx::mma_commit(&empty[used % L::kStages]);
+        for (int j = 0; j < n && ok; ++j) {
+          const uint32_t ev = used + 2 * j + 1, ek = ev + 1;
+          ok = wait_full(ev);
+          if (!ok) break;
+          if ((j + 1) * kKeys > it.klen) {
+            // Rows past the sequence hold the next one's values (or nothing): their weights are 0,
+            // but 0 * inf is not.
+            uint8_t* v = smem + L::kOffRing + (ev % L::kStages) * L::kTileBytes;
+            const int from = (it.klen - j * kKeys) * 128;
+            for (int b = 0; b < L::kBoxes; ++b)
+              for (int x = from + lane * 16; x < kBoxBytes; x += 512)
+                *reinterpret_cast<uint4*>(v + b * kBoxBytes + x) = make_uint4(0, 0, 0, 0);
+            ptx::fence_proxy_async_smem();
+            __syncwarp();
+          }
+          if (j + 1 < n) ok = wait_full(ek);
+          for (int i = 0; i < 2 && ok; ++i) {
+            const int ni = i ? it.n1 : it.n0;
+            if (j < ni) {
+              ok = wait(&p_ready[i], steps[i]++ & 1, kErrP);
+              if (ok && lane == 0) {
+                values(i, ev, j > 0);
+                if (j + 1 < ni) scores(i, ek, j + 2 == ni);
+              }
+            }
+          }
+          if (lane == 0) {
+            ptx::mma_commit(&empty[ev % L::kStages]);
+            if (j + 1 < n) ptx::mma_commit(&empty[ek % L::kStages]);
+          }
+          __syncwarp();
+        }
+        used += 2 * n;
+      }
+      // No product may still write tensor memory when it is freed.
+      if (lane == 0) {
+        ptx::mma_commit(drain);
+        volatile int never = 0;
+        ptx::mbar_wait(drain, 0, &never, kDrainLimitNs);
       }
       __syncwarp();
     }
-    // No product may still write tensor memory when it is freed.
-    if (lane == 0) {
-      ptx::mma_commit(drain);
-      volatile int never = 0;
-      ptx::mbar_wait(drain, 0, &never, kDrainLimitNs);
-    }
-    __syncwarp();
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsSoftmax));
     const int i = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
-    const int ni = i ? n1 : n0;
     const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem + lanes + i * kKeys, to = tmem + lanes + 256 + i * 128;
-    const int t0 = it.first + i * p.tile_tokens;
-    const int tok = t0 + row / p.group, g = row % p.group;
-    const bool mine = row < p.tile_tokens * p.group && tok < it.qlen;
-    const int limit = keys_of(p, it, tok);
-    const int least = keys_of(p, it, t0);      // no row of the tile sees fewer keys
-    float m = -INFINITY, l = 0.f;              // m in log2 units
+    const int row_tok = row / p.group, g = row % p.group;
+    const uint64_t scale2 = pair(p.scale_log2, p.scale_log2);
+    uint32_t steps = 0;
     bool ok = true;
-    for (int j = 0; j < ni; ++j) {
-      if (!ptx::mbar_wait(&s_full[i], j & 1, abort_flag, p.wait_limit_ns)) {
-        if (lane == 0) fail(p.err, abort_flag, kErrS);
-        ok = false;
-        break;
-      }
-      ptx::tc_fence_after();
-      uint32_t s[4][32];
+    Item it;
+    for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
+      const int ni = i ? it.n1 : it.n0;
+      const int t0 = it.first + i * p.tile_tokens;
+      const int tok = t0 + row_tok;
+      const bool mine = row_tok < p.tile_tokens && tok < it.qlen;
+      const int limit = keys_of(p, it, tok);
+      const int least = keys_of(p, it, t0);      // no row of the tile sees fewer keys
+      float m = -INFINITY;                       // in log2 units
+      uint64_t l2 = 0;                           // the sum, in two parts
+      for (int j = 0; j < ni; ++j, ++steps) {
+        if (!ptx::mbar_wait(&s_full[i], steps & 1, abort_flag, p.wait_limit_ns)) {
+          if (lane == 0) fail(p.err, abort_flag, kErrS);
+          ok = false;
+          break;
+        }
+        ptx::tc_fence_after();
+        uint32_t s[4][32];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
+        for (int c = 0; c < 4; ++c) ptx::tmem_ld_32x32b_x32(ts + c * 32, s[c]);
 #pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_wait_regs(s[c]);
-      if ((j + 1) * kKeys > least) {
-        const int seen = limit - j * kKeys;
+        for (int c = 0; c < 4; ++c) tmem_wait_regs(s[c]);
+        if ((j + 1) * kKeys > least) {
+          const int seen = limit - j * kKeys;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 4; ++c)
 #pragma unroll
-          for (int x = 0; x < 32; ++x)
-            if (c * 32 + x >= seen) s[c][x] = 0xff800000u;   // -infinity
-      }
-      float top = -INFINITY;
+            for (int x = 0; x < 32; ++x)
+              if (c * 32 + x >= seen) s[c][x] = 0xff800000u;   // -infinity
+        }
+        float tops[4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 4; ++c) {
+          tops[c] = max2(__uint_as_float(s[c][0]), __uint_as_float(s[c][1]));
 #pragma unroll
-        for (int x = 0; x < 32; ++x) top = fmaxf(top, __uint_as_float(s[c][x]));
-      top *= p.scale_log2;
-      if (__any_sync(0xffffffffu, top > m + kGrow || (m == -INFINITY && top > m))) {
-        const float now = fmaxf(m, top);
-        const float corr = now == m ? 1.f : exp2_fast(m - now);
-        m = now;
-        l *= corr;
-        if (j > 0) {
-          if (!ptx::mbar_wait(&o_done[i], (j - 1) & 1, abort_flag, p.wait_limit_ns)) {
-            if (lane == 0) fail(p.err, abort_flag, kErrO);
-            ok = false;
-            break;
+          for (int x = 2; x < 32; x += 2)
+            tops[c] = max3(tops[c], __uint_as_float(s[c][x]), __uint_as_float(s[c][x + 1]));
+        }
+        const float top = max2(max3(tops[0], tops[1], tops[2]), tops[3]) * p.scale_log2;
+        // (also where a NaN or an infinity makes the whole row NaN, whichever unit its weights take)
+        if (__any_sync(0xffffffffu, !(top <= m + kGrow))) {
+          const float now = max2(m, top);
+          const float corr = now == m ? 1.f : exp2_fast(m - now);
+          m = now == INFINITY ? NAN : now;
+          float la, lb;
+          unpair(l2, la, lb);
+          l2 = pair(la * corr, lb * corr);
+          if (j > 0) {
+            if (!ptx::mbar_wait(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+              if (lane == 0) fail(p.err, abort_flag, kErrO);
+              ok = false;
+              break;
+            }
+            ptx::tc_fence_after();
+#pragma unroll 1
+            for (int d = 0; d < p.dim; d += 32) {
+              uint32_t o[32];
+              ptx::tmem_ld_32x32b_x32(to + d, o);
+              tmem_wait_regs(o);
+#pragma unroll
+              for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
+              tmem_st_x32(to + d, o);
+            }
+            tmem_st_wait();
           }
-          ptx::tc_fence_after();
-          for (int d = 0; d < p.dim; d += 32) {
-            uint32_t o[32];
-            ptx::tmem_ld_32x32b_x32(to + d, o);
-            tmem_wait_regs(o);
+        }
+        const float off = m == -INFINITY ? 0.f : -m;
+        const uint64_t off2 = pair(off, off);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * corr);
-            tmem_st_x32(to + d, o);
+        for (int c = 0; c < 4; ++c) {
+          uint32_t w[16];
+#pragma unroll
+          for (int x = 0; x < 16; ++x) {
+            const uint64_t z2 = fma2(pair(__uint_as_float(s[c][2 * x]), __uint_as_float(s[c][2 * x + 1])),
+                                     scale2, off2);
+            float a, b;
+            if ((x + 1) * kPolyPairs / 16 != x * kPolyPairs / 16) {
+              exp2_poly<BF16>(z2, a, b);
+            } else {
+              unpair(z2, a, b);
+              a = exp2_fast(a);
+              b = exp2_fast(b);
+            }
+            l2 = add2(l2, pair(a, b));
+            w[x] = pack<BF16>(a, b);
           }
-          tmem_st_wait();
+          tmem_st_x16(ts + c * 16, w);
+        }
+        tmem_st_wait();
+        ptx::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&p_ready[i]);
+      }
+      const int64_t t = it.q0 + tok;
+      const int h = it.head * p.group + g;
+      uint16_t* out = p.out + t * p.out_token + h * p.out_head;
+      if (ok && ni > 0) {
+        if (!ptx::mbar_wait(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+          if (lane == 0) fail(p.err, abort_flag, kErrO);
+          ok = false;
         }
       }
-      const float off = m == -INFINITY ? 0.f : m;
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        uint32_t w[32];
-#pragma unroll
-        for (int x = 0; x < 32; ++x) {
-          const float a = exp2_fast(__uint_as_float(s[2 * c + x / 16][(2 * x) & 31]) * p.scale_log2 - off);
-          const float b = exp2_fast(__uint_as_float(s[2 * c + x / 16][(2 * x + 1) & 31]) * p.scale_log2 - off);
-          l += a + b;
-          w[x] = pack<BF16>(a, b);
-        }
-        tmem_st_x32(ts + c * 32, w);
-      }
-      tmem_st_wait();
-      ptx::tc_fence_before();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive(&p_ready[i]);
-    }
-    const int64_t t = it.q0 + tok;
-    const int h = it.head * p.group + g;
-    uint16_t* out = p.out + t * p.out_token + h * p.out_head;
-    if (ok && ni > 0) {
-      if (!ptx::mbar_wait(&o_done[i], (ni - 1) & 1, abort_flag, p.wait_limit_ns)) {
-        if (lane == 0) fail(p.err, abort_flag, kErrO);
-        ok = false;
-      }
-    }
-    if (ok) {
+      if (!ok) break;
       ptx::tc_fence_after();
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      float la, lb;
+      unpair(l2, la, lb);
+      const float l = la + lb;
+      const bool some = m != -INFINITY && limit > 0;
+      const float inv = 1.f / l;
+#pragma unroll 1
       for (int d = 0; d < p.dim; d += 32) {
         uint32_t o[32];
         if (ni > 0) {
@@ -457,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int x = 0; x < 32; x += 8) {
             if (d + x < p.dim) {
               uint32_t w[4] = {0, 0, 0, 0};
-              if (limit > 0)
+              if (some)
 #pragma unroll
                 for (int y = 0; y < 4; ++y)
                   w[y] = pack<BF16>(__uint_as_float(o[x + 2 * y]) * inv,
@@ -467,14 +676,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
+      ptx::tc_fence_before();                    // O is read before the next item's products write it
       if (mine && p.lse)
-        p.lse[t * p.heads + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
+        p.lse[t * p.heads + h] = some ? (m + log2f(l)) * 0.6931471805599453f : -INFINITY;
     }
   }
 
   ptx::tc_fence_before();
   __syncthreads();
-  if (warp == kSoftmaxWarps) {
+  if (warp == kMmaWarp) {
     ptx::tc_fence_after();
     ptx::tmem_dealloc(tmem, 512);
   }

@@ -82,6 +82,34 @@ __device__ __forceinline__ void griddep_wait() {
   asm volatile("griddepcontrol.wait;" ::: "memory");
 }
 
+// ------------------------------------------------------- cluster launch control
+// Ask to take over a CTA of this grid that has not started.  The 16-byte
+// answer lands at dst (16-byte aligned) and completes 16 bytes on `bar`.
+__device__ __forceinline__ void clc_try_cancel(void* dst, uint64_t* bar) {
+  asm volatile(
+      "clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128"
+      " [%0], [%1];" ::"r"(smem_addr(dst)),
+      "r"(smem_addr(bar))
+      : "memory");
+}
+// The answer: true and its blockIdx.x, or false when none is left (ask no
+// more then).
+__device__ __forceinline__ bool clc_answer(const void* src, int* block) {
+  uint32_t got, x = 0;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b128 r;\n\t"
+      "ld.shared.b128 r, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, r;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t"
+      "mov.u32 %1, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid::x.b32.b128 %1, r;\n\t}"
+      : "=r"(got), "=r"(x)
+      : "r"(smem_addr(src))
+      : "memory");
+  *block = static_cast<int>(x);
+  return got != 0;
+}
+
 // ---------------------------------------------------------------- clusters
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;
