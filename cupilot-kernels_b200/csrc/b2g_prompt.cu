@@ -47,9 +47,13 @@ constexpr int kThreads = 12 * 32;     // a whole third warpgroup, for the regist
 // Registers: 384 threads start with 168 each; the third warpgroup gives 96 of
 // each thread's to the softmax warps (2 * 128 * 216 + 128 * 72 = 384 * 168).
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
+constexpr int kAskAhead = 2;          // key tiles left to load when the next item is asked for
 constexpr int kItemReaders = kSoftmaxWarps + 2;
 // Of 16 pairs of exponentials, how many run on the FMA units.
-constexpr int kPolyPairs = 5;
+#ifndef POLY
+#define POLY 3
+#endif
+constexpr int kPolyPairs = POLY;
 constexpr float kGrow = 8.f;
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kBoxBytes = 128 * 128;  // 64 columns x 128 rows of 16 bits
@@ -64,7 +68,7 @@ struct Smem {
   static constexpr int kStages = DP == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;
   static constexpr int kOffBars = kOffRing + kStages * kTileBytes;
-  static constexpr int kNumBars = 2 * kStages + 2 * 5 + 4 + 2;
+  static constexpr int kNumBars = 2 * kStages + 2 * 6 + 4 + 3;
   static constexpr int kOffNext = (kOffBars + kNumBars * 8 + 15) / 16 * 16;   // 16-byte answer
   static constexpr int kOffItems = kOffNext + 16;
   static constexpr int kOffMisc = kOffItems + 2 * 48;
@@ -98,14 +102,33 @@ __device__ __forceinline__ void fail(int* err, volatile int* abort, int code) {
   *abort = 1;
 }
 
-// D += A B with A in tensor memory (16-bit pairs, 128 lanes).
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
-                                       uint32_t idesc, uint32_t accumulate) {
+// The halves of a shared-memory matrix descriptor (ptx::smem_desc) in the
+// 128-byte swizzle, rows of 8 x 128 bytes: the low one (address and leading
+// offset) moves with the tile, the high one is the same for all.  One thread
+// issues every product, between waits, so what it computes for each of them
+// counts: an addition.
+constexpr uint32_t kDescHigh = (1024u >> 4) | (1u << 14) | (ptx::kLayoutSw128 << 29);
+__device__ __forceinline__ uint32_t desc_low(uint32_t saddr, uint32_t lbo_bytes) {
+  return (saddr >> 4) | ((lbo_bytes >> 4) << 16);
+}
+// D (+)= A B^T, A and B in shared memory.
+__device__ __forceinline__ void mma_ss(uint32_t d_tmem, uint32_t a_low, uint32_t b_low, uint32_t idesc,
+                                       uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_low), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// D (+)= A B with A in tensor memory (16-bit pairs, 128 lanes).
+__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_low, uint32_t idesc,
+                                       uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "setp.ne.b32 p, %5, 0;\n\tmov.b64 b, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_low), "r"(kDescHigh), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 
@@ -284,12 +307,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = empty + L::kStages;     // [2]
   uint64_t* q_empty = q_full + 2;            // [2] the tile's last Q K^T has read Q
   uint64_t* s_full = q_full + 4;             // [2] S of the tile is complete
-  uint64_t* p_ready = q_full + 6;            // [2] P of the tile is stored
-  uint64_t* o_done = q_full + 8;             // [2] P V of the tile is added to O
-  uint64_t* item_full = q_full + 10;         // [2]
-  uint64_t* item_empty = q_full + 12;        // [2]
-  uint64_t* next_full = q_full + 14;
-  uint64_t* drain = q_full + 15;
+  uint64_t* p_half = q_full + 6;             // [2] P of the tile's first 64 keys is stored
+  uint64_t* p_ready = q_full + 8;            // [2] and that of the others
+  uint64_t* o_done = q_full + 10;            // [2] P V of the tile is added to O
+  uint64_t* item_full = q_full + 12;         // [2]
+  uint64_t* item_empty = q_full + 14;        // [2]
+  uint64_t* next_wanted = q_full + 16;       // the loads come to an item's end
+  uint64_t* next_full = q_full + 17;
+  uint64_t* drain = q_full + 18;
   uint8_t* next_answer = smem + L::kOffNext;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
@@ -305,11 +330,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       ptx::mbar_init(&q_full[i], 1);
       ptx::mbar_init(&q_empty[i], 1);
       ptx::mbar_init(&s_full[i], 1);
+      ptx::mbar_init(&p_half[i], kSoftmaxWarps / 2);
       ptx::mbar_init(&p_ready[i], kSoftmaxWarps / 2);
       ptx::mbar_init(&o_done[i], 1);
       ptx::mbar_init(&item_full[i], 1);
       ptx::mbar_init(&item_empty[i], kItemReaders);
     }
+    ptx::mbar_init(next_wanted, 1);
     ptx::mbar_init(next_full, 1);
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
@@ -326,7 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // The k-th item of this CTA, for the warps that work on it.
   auto get_item = [&](uint32_t k, Item* it) {
-    if (!ptx::mbar_wait(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns)) {
+    const bool come = ptx::mbar_wait(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns);
+    if (!__all_sync(0xffffffffu, come)) {
       if (lane == 0) fail(p.err, abort_flag, kErrItem);
       return false;
     }
@@ -344,38 +372,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       uint32_t k = 0, asked = 0;
       bool more = true;
       while (more) {
-        // Ask for another CTA's work now, use it when this item is handed out.
+        zero_rows(p, w, lane);
+        Item it;
+        // Late tiles see the most keys: they go first.
+        if (p.sequences > 0 && find_item(p, p.slots - 1 - w / p.kv_heads, w % p.kv_heads, &it)) {
+          it.more = 1;
+          if (!ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+            if (lane == 0) fail(p.err, abort_flag, kErrItem);
+            break;
+          }
+          if (lane == 0) {
+            *item_at(k) = it;
+            ptx::mbar_arrive(&item_full[k & 1]);
+          }
+          // Another CTA's work is taken over when this item's last key tiles are on their way: early
+          // enough to hide the question, late enough that whoever is done first takes what is left.
+          if (!ptx::mbar_wait(next_wanted, k & 1, abort_flag, p.wait_limit_ns)) {
+            if (lane == 0) fail(p.err, abort_flag, kErrNext);
+            break;
+          }
+          ++k;
+        }
         if (lane == 0) {
           ptx::fence_proxy_async_smem();
           ptx::mbar_arrive_expect_tx(next_full, 16);
           ptx::clc_try_cancel(next_answer, next_full);
         }
-        zero_rows(p, w, lane);
-        Item it;
-        // Late tiles see the most keys: they go first.
-        bool work = p.sequences > 0 && find_item(p, p.slots - 1 - w / p.kv_heads, w % p.kv_heads, &it);
-        if (work) {
-          if (!ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
-            if (lane == 0) fail(p.err, abort_flag, kErrItem);
-            more = false;
-          } else {
-            it.more = 1;
-            if (lane == 0) {
-              *item_at(k) = it;
-              ptx::mbar_arrive(&item_full[k & 1]);
-            }
-            ++k;
-          }
-        }
-        // (waited for even after a failure: the answer has to land before the CTA leaves)
-        volatile int never = 0;
+        volatile int never = 0;                  // (the answer lands before the CTA leaves)
         if (!ptx::mbar_wait(next_full, asked & 1, &never, p.wait_limit_ns)) {
           if (lane == 0) fail(p.err, abort_flag, kErrNext);
-          more = false;
-        } else if (!ptx::clc_answer(next_answer, &w)) {
-          more = false;
+          break;
         }
         ++asked;
+        more = ptx::clc_answer(next_answer, &w);
         __syncwarp();
       }
       if (ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
@@ -397,7 +426,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       Item it;
       for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
-        if (lane == 0) {
+        if (ptx::elect_one()) {
           auto load_q = [&](int i) {
             if (!ptx::mbar_wait(&q_empty[i], (q_issued[i] & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
               fail(p.err, abort_flag, kErrEmpty);
@@ -428,12 +457,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (n > 0) ok = ok && load_kv(&map_k, 0);
           if (it.n1 > 0) ok = ok && load_q(1);
           if (n > 0) ok = ok && load_kv(&map_v, 0);
-          for (int j = 1; j < n && ok; ++j) ok = load_kv(&map_k, j) && load_kv(&map_v, j);
+          const int ask = max(n - kAskAhead, 0);
+          if (ask == 0) ptx::mbar_arrive(next_wanted);
+          for (int j = 1; j < n && ok; ++j) {
+            if (j == ask) ptx::mbar_arrive(next_wanted);
+            ok = load_kv(&map_k, j) && load_kv(&map_v, j);
+          }
         }
-        ok = __shfl_sync(0xffffffffu, ok, 0);
+        ok = __all_sync(0xffffffffu, ok);
       }
       // Every load has landed before the CTA may leave.
-      if (lane == 0) {
+      if (ptx::elect_one()) {
         volatile int never = 0;
         for (int i = 0; i < 2; ++i)
           if (q_issued[i]) ptx::mbar_wait(&q_full[i], (q_issued[i] - 1) & 1, &never, kDrainLimitNs);
@@ -446,11 +480,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
       const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
       const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
-      const uint32_t ring = ptx::smem_addr(smem + L::kOffRing);
+      const uint32_t q_low = desc_low(ptx::smem_addr(smem), 16);
+      const uint32_t k_low = desc_low(ptx::smem_addr(smem + L::kOffRing), 16);
+      const uint32_t v_low = desc_low(ptx::smem_addr(smem + L::kOffRing), kBoxBytes);
       uint32_t q_used[2] = {0, 0}, steps[2] = {0, 0}, used = 0;
       bool ok = true;
+      // (one answer for the warp: it stays converged)
       auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        if (!ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns)) {
+        const bool come = ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns);
+        if (!__all_sync(0xffffffffu, come)) {
           if (lane == 0) fail(p.err, abort_flag, code);
           return false;
         }
@@ -461,24 +499,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         return wait(&full[e % L::kStages], (e / L::kStages) & 1, kErrFull);
       };
       auto scores = [&](int i, uint32_t e, bool last) {      // S_i = Q_i K^T, K in ring entry e
-        const uint32_t sq = ptx::smem_addr(smem + i * L::kTileBytes);
-        const uint32_t sk = ring + (e % L::kStages) * L::kTileBytes;
-        for (int k = 0; k < p.dim / 16; ++k) {
-          const uint32_t at = (k >> 2) * kBoxBytes + (k & 3) * 32;
-          ptx::mma_f16(tmem + i * kKeys, ptx::smem_desc(sq + at, 16, 1024, ptx::kLayoutSw128),
-                       ptx::smem_desc(sk + at, 16, 1024, ptx::kLayoutSw128), idesc_s, k > 0);
+        const uint32_t sq = q_low + i * (L::kTileBytes >> 4);
+        const uint32_t sk = k_low + (e % L::kStages) * (L::kTileBytes >> 4);
+#pragma unroll
+        for (int k = 0; k < DP / 16; ++k) {
+          const uint32_t at = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
+          if (k * 16 < p.dim) mma_ss(tmem + i * kKeys, sq + at, sk + at, idesc_s, k > 0);
         }
         ptx::mma_commit(&s_full[i]);
         if (last) ptx::mma_commit(&q_empty[i]);
       };
-      auto values = [&](int i, uint32_t e, bool add) {   // O_i += P_i V, V in ring entry e
-        const uint32_t sv = ring + (e % L::kStages) * L::kTileBytes;
+      auto values = [&](int i, uint32_t e, int half, bool add) {   // O_i += P_i V, V in ring entry e
+        const uint32_t sv = v_low + (e % L::kStages) * (L::kTileBytes >> 4);
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)
-          mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8,
-                 ptx::smem_desc(sv + k * 16 * 128, kBoxBytes, 1024, ptx::kLayoutSw128), idesc_o,
-                 add || k > 0);
-        ptx::mma_commit(&o_done[i]);
+        for (int x = 0; x < kKeys / 32; ++x) {
+          const int k = half * (kKeys / 32) + x;
+          mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8, sv + k * (16 * 128 >> 4), idesc_o,
+                 add || x > 0);
+        }
+        if (half) ptx::mma_commit(&o_done[i]);
       };
       Item it;
       for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
@@ -489,9 +528,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int ni = i ? it.n1 : it.n0;
           if (ni == 0) continue;
           ok = wait(&q_full[i], q_used[i]++ & 1, kErrQ);
-          if (ok && lane == 0) scores(i, used, ni == 1);
+          if (ok && ptx::elect_one()) scores(i, used, ni == 1);
         }
-        if (lane == 0) ptx::mma_commit(&empty[used % L::kStages]);
+        if (ptx::elect_one()) ptx::mma_commit(&empty[used % L::kStages]);
         for (int j = 0; j < n && ok; ++j) {
           const uint32_t ev = used + 2 * j + 1, ek = ev + 1;
           ok = wait_full(ev);
@@ -511,14 +550,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int i = 0; i < 2 && ok; ++i) {
             const int ni = i ? it.n1 : it.n0;
             if (j < ni) {
-              ok = wait(&p_ready[i], steps[i]++ & 1, kErrP);
-              if (ok && lane == 0) {
-                values(i, ev, j > 0);
+              ok = wait(&p_half[i], steps[i] & 1, kErrP);
+              if (ok && ptx::elect_one()) values(i, ev, 0, j > 0);
+              ok = ok && wait(&p_ready[i], steps[i]++ & 1, kErrP);
+              if (ok && ptx::elect_one()) {
+                values(i, ev, 1, true);
                 if (j + 1 < ni) scores(i, ek, j + 2 == ni);
               }
             }
           }
-          if (lane == 0) {
+          if (ptx::elect_one()) {
             ptx::mma_commit(&empty[ev % L::kStages]);
             if (j + 1 < n) ptx::mma_commit(&empty[ek % L::kStages]);
           }
@@ -527,7 +568,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         used += 2 * n;
       }
       // No product may still write tensor memory when it is freed.
-      if (lane == 0) {
+      __syncwarp();
+      if (ptx::elect_one()) {
         ptx::mma_commit(drain);
         volatile int never = 0;
         ptx::mbar_wait(drain, 0, &never, kDrainLimitNs);
@@ -632,11 +674,13 @@ __global__ void __launch_bounds__(kThreads, 1)
             w[x] = pack<BF16>(a, b);
           }
           tmem_st_x16(ts + c * 16, w);
+          if (c & 1) {
+            tmem_st_wait();
+            ptx::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) ptx::mbar_arrive(c == 1 ? &p_half[i] : &p_ready[i]);
+          }
         }
-        tmem_st_wait();
-        ptx::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) ptx::mbar_arrive(&p_ready[i]);
       }
       const int64_t t = it.q0 + tok;
       const int h = it.head * p.group + g;
