@@ -512,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
             vs = __ldg(a.v_scale + static_cast<int64_t>(id) * a.kv_heads + head);
           }
         }
-        if (!ptx::mbar_wait(&empty[slot], ((n / L::kStages) & 1) ^ 1, abort_flag, a.wait_limit_ns)) {
+        if (!ptx::mbar_wait_suspended(&empty[slot], ((n / L::kStages) & 1) ^ 1, abort_flag, a.wait_limit_ns)) {
           if (lane == 0) fail(a.err, abort_flag, kErrEmpty);
           ok = false;
           break;
@@ -541,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     // Every load has landed before the CTA may leave (at once, but after a failure).
     volatile int never = 0;
     for (uint32_t e = n > L::kStages ? n - L::kStages : 0; e < n; ++e)
-      ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
+      ptx::mbar_wait_suspended(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
     return;
   }
 
@@ -564,7 +564,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     load_query<DP, ROWS, E4M3>(s, a, seg.r, head, rg, lane);
     for (int t = seg.t0; t < seg.t1; ++t, ++n) {
       const int slot = n % L::kStages;
-      if (!ptx::mbar_wait(&full[slot], (n / L::kStages) & 1, abort_flag, a.wait_limit_ns)) {
+      if (!ptx::mbar_wait_suspended(&full[slot], (n / L::kStages) & 1, abort_flag, a.wait_limit_ns)) {
         if (lane == 0) fail(a.err, abort_flag, kErrFull);
         break;
       }

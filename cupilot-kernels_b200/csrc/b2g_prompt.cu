@@ -18,6 +18,7 @@
 //                    tile's P V and next Q K^T keep the tensor cores busy
 //   warp 9           TMA loads: Q, then K and V tiles through a ring
 //   warp 10          the next work item
+//   warp 11          clears the rows of a V tile past the end of its sequence
 // The maximum is taken over only where it grew by more than 2^8 (P stays
 // within 16 bits' range, l and O are fp32): then, rarely, the softmax warps
 // rescale O themselves.
@@ -42,13 +43,13 @@ namespace prompt {
 constexpr int kRows = 128;            // rows of a tile
 constexpr int kKeys = 128;            // keys of a tile
 constexpr int kSoftmaxWarps = 8;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kNextWarp = 10;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kNextWarp = 10, kTailWarp = 11;
 constexpr int kThreads = 12 * 32;     // a whole third warpgroup, for the register split
 // Registers: 384 threads start with 168 each; the third warpgroup gives 96 of
 // each thread's to the softmax warps (2 * 128 * 216 + 128 * 72 = 384 * 168).
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kAskAhead = 2;          // key tiles left to load when the next item is asked for
-constexpr int kItemReaders = kSoftmaxWarps + 2;
+constexpr int kItemReaders = kSoftmaxWarps + 3;
 // Of 16 pairs of exponentials, how many run on the FMA units.
 #ifndef POLY
 #define POLY 3
@@ -68,7 +69,7 @@ struct Smem {
   static constexpr int kStages = DP == 128 ? 5 : 8;
   static constexpr int kOffRing = 2 * kTileBytes;
   static constexpr int kOffBars = kOffRing + kStages * kTileBytes;
-  static constexpr int kNumBars = 2 * kStages + 2 * 6 + 4 + 3;
+  static constexpr int kNumBars = 2 * kStages + 2 * 6 + 4 + 5;
   static constexpr int kOffNext = (kOffBars + kNumBars * 8 + 15) / 16 * 16;   // 16-byte answer
   static constexpr int kOffItems = kOffNext + 16;
   static constexpr int kOffMisc = kOffItems + 2 * 48;
@@ -314,7 +315,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* item_empty = q_full + 14;        // [2]
   uint64_t* next_wanted = q_full + 16;       // the loads come to an item's end
   uint64_t* next_full = q_full + 17;
-  uint64_t* drain = q_full + 18;
+  uint64_t* tail_there = q_full + 18;        // the item's last V tile, of a sequence that ends in it
+  uint64_t* tail_done = q_full + 19;         // it is cleared past the sequence
+  uint64_t* drain = q_full + 20;
   uint8_t* next_answer = smem + L::kOffNext;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kOffMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kOffMisc + 4);
@@ -338,6 +341,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     ptx::mbar_init(next_wanted, 1);
     ptx::mbar_init(next_full, 1);
+    ptx::mbar_init(tail_there, 1);
+    ptx::mbar_init(tail_done, 1);
     ptx::mbar_init(drain, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
@@ -353,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   // The k-th item of this CTA, for the warps that work on it.
   auto get_item = [&](uint32_t k, Item* it) {
-    const bool come = ptx::mbar_wait(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns);
+    const bool come = ptx::mbar_wait_suspended(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns);
     if (!__all_sync(0xffffffffu, come)) {
       if (lane == 0) fail(p.err, abort_flag, kErrItem);
       return false;
@@ -377,7 +382,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Late tiles see the most keys: they go first.
         if (p.sequences > 0 && find_item(p, p.slots - 1 - w / p.kv_heads, w % p.kv_heads, &it)) {
           it.more = 1;
-          if (!ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+          if (!ptx::mbar_wait_suspended(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
             if (lane == 0) fail(p.err, abort_flag, kErrItem);
             break;
           }
@@ -387,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // Another CTA's work is taken over when this item's last key tiles are on their way: early
           // enough to hide the question, late enough that whoever is done first takes what is left.
-          if (!ptx::mbar_wait(next_wanted, k & 1, abort_flag, p.wait_limit_ns)) {
+          if (!ptx::mbar_wait_suspended(next_wanted, k & 1, abort_flag, p.wait_limit_ns)) {
             if (lane == 0) fail(p.err, abort_flag, kErrNext);
             break;
           }
@@ -399,7 +404,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::clc_try_cancel(next_answer, next_full);
         }
         volatile int never = 0;                  // (the answer lands before the CTA leaves)
-        if (!ptx::mbar_wait(next_full, asked & 1, &never, p.wait_limit_ns)) {
+        if (!ptx::mbar_wait_suspended(next_full, asked & 1, &never, p.wait_limit_ns)) {
           if (lane == 0) fail(p.err, abort_flag, kErrNext);
           break;
         }
@@ -407,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         more = ptx::clc_answer(next_answer, &w);
         __syncwarp();
       }
-      if (ptx::mbar_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+      if (ptx::mbar_wait_suspended(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
         if (lane == 0) {
           item_at(k)->more = 0;
           ptx::mbar_arrive(&item_full[k & 1]);
@@ -428,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
         if (ptx::elect_one()) {
           auto load_q = [&](int i) {
-            if (!ptx::mbar_wait(&q_empty[i], (q_issued[i] & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+            if (!ptx::mbar_wait_suspended(&q_empty[i], (q_issued[i] & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
               fail(p.err, abort_flag, kErrEmpty);
               return false;
             }
@@ -441,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           };
           auto load_kv = [&](const CUtensorMap* map, int j) {
             const uint32_t s = issued % L::kStages;
-            if (!ptx::mbar_wait(&empty[s], ((issued / L::kStages) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+            if (!ptx::mbar_wait_suspended(&empty[s], ((issued / L::kStages) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
               fail(p.err, abort_flag, kErrEmpty);
               return false;
             }
@@ -470,106 +475,146 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (ptx::elect_one()) {
         volatile int never = 0;
         for (int i = 0; i < 2; ++i)
-          if (q_issued[i]) ptx::mbar_wait(&q_full[i], (q_issued[i] - 1) & 1, &never, kDrainLimitNs);
+          if (q_issued[i]) ptx::mbar_wait_suspended(&q_full[i], (q_issued[i] - 1) & 1, &never, kDrainLimitNs);
         for (uint32_t e = issued > L::kStages ? issued - L::kStages : 0; e < issued; ++e)
-          ptx::mbar_wait(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
+          ptx::mbar_wait_suspended(&full[e % L::kStages], (e / L::kStages) & 1, &never, kDrainLimitNs);
       }
       __syncwarp();
-    } else if (warp == kMmaWarp) {
-      // ---------------------------------------------------------- products
-      constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
-      const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
-      const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
-      const uint32_t q_low = desc_low(ptx::smem_addr(smem), 16);
-      const uint32_t k_low = desc_low(ptx::smem_addr(smem + L::kOffRing), 16);
-      const uint32_t v_low = desc_low(ptx::smem_addr(smem + L::kOffRing), kBoxBytes);
-      uint32_t q_used[2] = {0, 0}, steps[2] = {0, 0}, used = 0;
-      bool ok = true;
-      // (one answer for the warp: it stays converged)
-      auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
-        const bool come = ptx::mbar_wait(bar, parity, abort_flag, p.wait_limit_ns);
-        if (!__all_sync(0xffffffffu, come)) {
-          if (lane == 0) fail(p.err, abort_flag, code);
-          return false;
-        }
-        ptx::tc_fence_after();
-        return true;
-      };
-      auto wait_full = [&](uint32_t e) {
-        return wait(&full[e % L::kStages], (e / L::kStages) & 1, kErrFull);
-      };
-      auto scores = [&](int i, uint32_t e, bool last) {      // S_i = Q_i K^T, K in ring entry e
-        const uint32_t sq = q_low + i * (L::kTileBytes >> 4);
-        const uint32_t sk = k_low + (e % L::kStages) * (L::kTileBytes >> 4);
-#pragma unroll
-        for (int k = 0; k < DP / 16; ++k) {
-          const uint32_t at = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
-          if (k * 16 < p.dim) mma_ss(tmem + i * kKeys, sq + at, sk + at, idesc_s, k > 0);
-        }
-        ptx::mma_commit(&s_full[i]);
-        if (last) ptx::mma_commit(&q_empty[i]);
-      };
-      auto values = [&](int i, uint32_t e, int half, bool add) {   // O_i += P_i V, V in ring entry e
-        const uint32_t sv = v_low + (e % L::kStages) * (L::kTileBytes >> 4);
-#pragma unroll
-        for (int x = 0; x < kKeys / 32; ++x) {
-          const int k = half * (kKeys / 32) + x;
-          mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8, sv + k * (16 * 128 >> 4), idesc_o,
-                 add || x > 0);
-        }
-        if (half) ptx::mma_commit(&o_done[i]);
-      };
+    } else if (warp == kTailWarp) {
+      // ---------------------------------------------------------- tails
+      // Rows of a V tile past its sequence hold the next one's values (or nothing): their weights
+      // are 0, but 0 * inf is not.  They are cleared before the products read them.
+      uint32_t used = 0, tails = 0;
       Item it;
+      bool ok = true;
       for (uint32_t k = 0; ok && get_item(k, &it); ++k) {
         const int n = max(it.n0, it.n1);
-        if (n == 0) continue;
-        ok = wait_full(used);
-        for (int i = 0; i < 2 && ok; ++i) {
-          const int ni = i ? it.n1 : it.n0;
-          if (ni == 0) continue;
-          ok = wait(&q_full[i], q_used[i]++ & 1, kErrQ);
-          if (ok && ptx::elect_one()) scores(i, used, ni == 1);
-        }
-        if (ptx::elect_one()) ptx::mma_commit(&empty[used % L::kStages]);
-        for (int j = 0; j < n && ok; ++j) {
-          const uint32_t ev = used + 2 * j + 1, ek = ev + 1;
-          ok = wait_full(ev);
-          if (!ok) break;
-          if ((j + 1) * kKeys > it.klen) {
-            // Rows past the sequence hold the next one's values (or nothing): their weights are 0,
-            // but 0 * inf is not.
-            uint8_t* v = smem + L::kOffRing + (ev % L::kStages) * L::kTileBytes;
-            const int from = (it.klen - j * kKeys) * 128;
-            for (int b = 0; b < L::kBoxes; ++b)
-              for (int x = from + lane * 16; x < kBoxBytes; x += 512)
-                *reinterpret_cast<uint4*>(v + b * kBoxBytes + x) = make_uint4(0, 0, 0, 0);
-            ptx::fence_proxy_async_smem();
-            __syncwarp();
+        if (n * kKeys > it.klen) {
+          const uint32_t e = used + 2 * (n - 1) + 1;
+          const bool come = ptx::mbar_wait_suspended(tail_there, tails++ & 1, abort_flag, p.wait_limit_ns);
+          if (!__all_sync(0xffffffffu, come)) {
+            if (lane == 0) fail(p.err, abort_flag, kErrFull);
+            ok = false;
+            break;
           }
-          if (j + 1 < n) ok = wait_full(ek);
-          for (int i = 0; i < 2 && ok; ++i) {
-            const int ni = i ? it.n1 : it.n0;
-            if (j < ni) {
-              ok = wait(&p_half[i], steps[i] & 1, kErrP);
-              if (ok && ptx::elect_one()) values(i, ev, 0, j > 0);
-              ok = ok && wait(&p_ready[i], steps[i]++ & 1, kErrP);
-              if (ok && ptx::elect_one()) {
-                values(i, ev, 1, true);
-                if (j + 1 < ni) scores(i, ek, j + 2 == ni);
-              }
-            }
-          }
-          if (ptx::elect_one()) {
-            ptx::mma_commit(&empty[ev % L::kStages]);
-            if (j + 1 < n) ptx::mma_commit(&empty[ek % L::kStages]);
-          }
+          uint8_t* v = smem + L::kOffRing + (e % L::kStages) * L::kTileBytes;
+          const int from = (it.klen - (n - 1) * kKeys) * 128;
+          for (int b = 0; b < L::kBoxes; ++b)
+            for (int x = from + lane * 16; x < kBoxBytes; x += 512)
+              *reinterpret_cast<uint4*>(v + b * kBoxBytes + x) = make_uint4(0, 0, 0, 0);
+          ptx::fence_proxy_async_smem();
           __syncwarp();
+          if (lane == 0) ptx::mbar_arrive(tail_done);
         }
         used += 2 * n;
       }
-      // No product may still write tensor memory when it is freed.
-      __syncwarp();
+    } else if (warp == kMmaWarp) {
+      // ---------------------------------------------------------- products
+      // One thread does it all, and between two products of a tile pair its own instructions are
+      // what the tensor cores wait for: barriers by shared address, ring positions that move on
+      // without a division, the next tiles' arrival looked at while a softmax still runs.
+      constexpr uint32_t kType = BF16 ? (1u << 7) | (1u << 10) : 0u;
+      const uint32_t idesc_s = ptx::idesc_f16(kRows, kKeys, false, false) | kType;
+      const uint32_t idesc_o = ptx::idesc_f16(kRows, p.dim, false, true) | kType;
+      constexpr uint32_t kTileLow = L::kTileBytes >> 4;
+      const uint32_t q_low = desc_low(ptx::smem_addr(smem), 16);
+      const uint32_t k_low = desc_low(ptx::smem_addr(smem + L::kOffRing), 16);
+      const uint32_t v_low = desc_low(ptx::smem_addr(smem + L::kOffRing), kBoxBytes);
       if (ptx::elect_one()) {
+        bool ok = true;
+        auto wait = [&](uint64_t* bar, uint32_t parity, int code) {
+          if (!ptx::mbar_wait_suspended(bar, parity, abort_flag, p.wait_limit_ns)) {
+            fail(p.err, abort_flag, code);
+            ok = false;
+          }
+        };
+        uint32_t slot = 0, ring_phase = 0;     // of the next ring entry
+        // Waits for the next ring entry; its slot.
+        auto take = [&]() {
+          const uint32_t at = slot;
+          wait(&full[at], ring_phase, kErrFull);
+          if (++slot == L::kStages) slot = 0, ring_phase ^= 1;
+          return at;
+        };
+        auto scores = [&](int i, uint32_t at, bool last) {      // S_i = Q_i K^T, K in ring slot `at`
+          const uint32_t sq = q_low + i * kTileLow, sk = k_low + at * kTileLow;
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k) {
+            const uint32_t off = ((k >> 2) * kBoxBytes + (k & 3) * 32) >> 4;
+            if (k * 16 < p.dim) mma_ss(tmem + i * kKeys, sq + off, sk + off, idesc_s, k > 0);
+          }
+          ptx::mma_commit(&s_full[i]);
+          if (last) ptx::mma_commit(&q_empty[i]);
+        };
+        auto values = [&](int i, uint32_t at, int half, bool add) {   // O_i += P_i V, V in slot `at`
+          const uint32_t sv = v_low + at * kTileLow;
+#pragma unroll
+          for (int x = 0; x < kKeys / 32; ++x) {
+            const int k = half * (kKeys / 32) + x;
+            mma_ts(tmem + 256 + i * 128, tmem + i * kKeys + k * 8, sv + k * (16 * 128 >> 4), idesc_o,
+                   add || x > 0);
+          }
+          if (half) ptx::mma_commit(&o_done[i]);
+        };
+        uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0}, tail_phase = 0;
+        for (uint32_t k = 0; ok; ++k) {
+          wait(&item_full[k & 1], (k >> 1) & 1, kErrItem);
+          if (!ok) break;
+          const Item* it = item_at(k);
+          const int n0 = it->n0, n1 = it->n1, klen = it->klen, more = it->more;
+          ptx::mbar_arrive(&item_empty[k & 1]);
+          if (!more) break;
+          const int n = max(n0, n1);
+          if (n == 0) continue;
+          const bool tail = n * kKeys > klen;
+          const uint32_t first = take();
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int ni = i ? n1 : n0;
+            if (ni > 0 && ok) {
+              wait(&q_full[i], q_phase[i], kErrQ);
+              q_phase[i] ^= 1;
+              if (ok) scores(i, first, ni == 1);
+            }
+          }
+          ptx::mma_commit(&empty[first]);
+          uint32_t v = take();
+          if (tail && n == 1) ptx::mbar_arrive(tail_there);
+          uint32_t kk = n > 1 ? take() : 0;
+          for (int j = 0; j < n && ok; ++j) {
+            if (tail && j == n - 1) {
+              wait(tail_done, tail_phase, kErrFull);
+              tail_phase ^= 1;
+            }
+            uint32_t v_next = 0, k_next = 0;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int ni = i ? n1 : n0;
+              if (j < ni && ok) {
+                wait(&p_half[i], p_phase[i], kErrP);
+                ptx::tc_fence_after();
+                if (ok) values(i, v, 0, j > 0);
+                wait(&p_ready[i], p_phase[i], kErrP);
+                p_phase[i] ^= 1;
+                ptx::tc_fence_after();
+                if (ok) {
+                  values(i, v, 1, true);
+                  if (j + 1 < ni) scores(i, kk, j + 2 == ni);
+                }
+              }
+              if (i == 0 && ok) {
+                if (j + 1 < n) v_next = take();
+                if (tail && j + 2 == n) ptx::mbar_arrive(tail_there);
+                if (j + 2 < n) k_next = take();
+              }
+            }
+            ptx::mma_commit(&empty[v]);
+            if (j + 1 < n) ptx::mma_commit(&empty[kk]);
+            v = v_next;
+            kk = k_next;
+          }
+        }
+        // No product may still write tensor memory when it is freed.
         ptx::mma_commit(drain);
         volatile int never = 0;
         ptx::mbar_wait(drain, 0, &never, kDrainLimitNs);
@@ -598,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY;                       // in log2 units
       uint64_t l2 = 0;                           // the sum, in two parts
       for (int j = 0; j < ni; ++j, ++steps) {
-        if (!ptx::mbar_wait(&s_full[i], steps & 1, abort_flag, p.wait_limit_ns)) {
+        if (!ptx::mbar_wait_suspended(&s_full[i], steps & 1, abort_flag, p.wait_limit_ns)) {
           if (lane == 0) fail(p.err, abort_flag, kErrS);
           ok = false;
           break;
@@ -635,7 +680,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           unpair(l2, la, lb);
           l2 = pair(la * corr, lb * corr);
           if (j > 0) {
-            if (!ptx::mbar_wait(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+            if (!ptx::mbar_wait_suspended(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
               if (lane == 0) fail(p.err, abort_flag, kErrO);
               ok = false;
               break;
@@ -686,7 +731,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int h = it.head * p.group + g;
       uint16_t* out = p.out + t * p.out_token + h * p.out_head;
       if (ok && ni > 0) {
-        if (!ptx::mbar_wait(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+        if (!ptx::mbar_wait_suspended(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
           if (lane == 0) fail(p.err, abort_flag, kErrO);
           ok = false;
         }
