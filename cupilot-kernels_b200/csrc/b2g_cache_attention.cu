@@ -43,6 +43,7 @@ constexpr int kThreads = (kWarps + 1) * 32;     // and the producer
 constexpr int kTile = 16 * kWarps;              // tokens of a stage, 16 a consumer warp
 constexpr float kGrow = 8.f;           // a maximum may be passed by 2^8 before the sums are rescaled
 constexpr uint64_t kDrainLimitNs = 100000000ull;
+constexpr int kJoin = 4;                     // rows of parts that a joining warp loads at once
 constexpr uint32_t kNoBlock = 0xffffffffu;   // in the place of a key scale
 enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
 
@@ -445,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     ptx::fence_mbar_init();
   }
 
+  ptx::griddep_wait();
   int lo, hi, run;
   const int total = scan_tiles(a, warp_sum, &lo, &hi, &run);
   Segments seg;
@@ -518,14 +520,10 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
           break;
         }
         const int first = (t - had_tile) * kWarps;       // lane of the stage's first piece
-        if (lane >= first && lane < first + kWarps)
-          // A block outside the cache leaves its tokens out.
-          scales[slot * kWarps + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
-        __syncwarp();
         const int box_id = __shfl_sync(0xffffffffu, id, (first + lane * box_pieces) & 31);
         const bool load = lane < boxes && box_id >= 0;
         const unsigned loads = __ballot_sync(0xffffffffu, load);
-        if (lane == 0) ptx::mbar_arrive_expect_tx(&full[slot], __popc(loads) * 2 * box_bytes);
+        if (lane == 0) ptx::mbar_expect_tx(&full[slot], __popc(loads) * 2 * box_bytes);
         __syncwarp();
         if (load) {
           uint8_t* to = smem + slot * L::kStageBytes + lane * box_bytes;
@@ -534,6 +532,12 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
           ptx::tma_load_2d(to, &map_k, &full[slot], 0, y);
           ptx::tma_load_2d(to + L::kSideBytes, &map_v, &full[slot], 0, y);
         }
+        // The scales, which may still be on their way, complete the stage.
+        if (lane >= first && lane < first + kWarps)
+          // A block outside the cache leaves its tokens out.
+          scales[slot * kWarps + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive(&full[slot]);
         __syncwarp();
         ++n;
       }
@@ -638,6 +642,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
 template <int DP, int ROWS>
 __global__ void cache_join_kernel(const Args a) {
   extern __shared__ float sm[];          // [warps][DP + 1]
+  ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int heads = a.kv_heads * a.row_groups;
   const int j = blockIdx.x % (a.kv_heads * a.group), r = blockIdx.x / (a.kv_heads * a.group);
@@ -664,17 +669,38 @@ __global__ void cache_join_kernel(const Args a) {
   for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_m[slot_of(c)]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+  // A warp's parts: their weights side by side in the lanes, their rows kJoin at a time.
   float l = 0.f, acc[DP / 32];
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
-  for (int c = c0 + warp; c <= c1; c += warps) {
-    const int64_t slot = slot_of(c);
-    const float pm = a.part_m[slot];
-    const float e = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
-    l += e * a.part_l[slot];
+  for (int base = c0 + warp; base <= c1; base += 32 * warps) {
+    const int own = base + lane * warps;
+    float e = 0.f;
+    if (own <= c1) {
+      const float pm = a.part_m[slot_of(own)];
+      e = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
+      l += e * a.part_l[slot_of(own)];
+    }
+    const int n = min(32, (c1 - base) / warps + 1);
+    for (int k = 0; k < n; k += kJoin) {
+      float v[kJoin][DP / 32];
 #pragma unroll
-    for (int i = 0; i < DP / 32; ++i) acc[i] += e * a.part_o[slot * DP + lane + 32 * i];
+      for (int x = 0; x < kJoin; ++x) {
+        const int64_t slot = slot_of(base + (k + x) * warps);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i)
+          v[x][i] = k + x < n ? a.part_o[slot * DP + lane + 32 * i] : 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < kJoin; ++x) {
+        const float w = __shfl_sync(0xffffffffu, e, (k + x) & 31);
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) acc[i] += (k + x < n ? w : 0.f) * v[x][i];
+      }
+    }
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
 #pragma unroll
   for (int i = 0; i < DP / 32; ++i) sm[warp * (DP + 1) + lane + 32 * i] = acc[i];
   if (lane == 0) sm[warp * (DP + 1) + DP] = l;
@@ -751,21 +777,26 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
       return B2G_ERR_LAUNCH;
     configured = dev;
   }
-  cache_attention_kernel<DP, ROWS, E4M3><<<a.grid, kThreads, L::kBytes, stream>>>(mk, mv, a);
-  if (cudaGetLastError() != cudaSuccess) return B2G_ERR_LAUNCH;
-  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-  // Parts of a head, were all lengths alike.
-  const int warps = a.grid > 16 * a.requests * a.kv_heads * a.row_groups ? 16 : 4;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(a.requests * heads), 1, 1);
-  cfg.blockDim = dim3(warps * 32, 1, 1);
-  cfg.dynamicSmemBytes = warps * (DP + 1) * sizeof(float);
-  cfg.stream = stream;
+  // Both kernels may be set up while the one before them on the stream still runs; they wait for it
+  // before they touch memory.
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(a.grid), 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = L::kBytes;
+  cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = b2g::pdl_enabled() ? 1 : 0;
+  if (cudaLaunchKernelEx(&cfg, cache_attention_kernel<DP, ROWS, E4M3>, mk, mv, a) != cudaSuccess)
+    return B2G_ERR_LAUNCH;
+  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
+  // Parts of a head, were all lengths alike.
+  const int warps = a.grid > 16 * a.requests * a.kv_heads * a.row_groups ? 16 : 4;
+  cfg.gridDim = dim3(static_cast<unsigned>(a.requests * heads), 1, 1);
+  cfg.blockDim = dim3(warps * 32, 1, 1);
+  cfg.dynamicSmemBytes = warps * (DP + 1) * sizeof(float);
   if (cudaLaunchKernelEx(&cfg, cache_join_kernel<DP, ROWS>, a) != cudaSuccess) return B2G_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }
