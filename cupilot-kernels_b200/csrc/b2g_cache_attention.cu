@@ -40,7 +40,10 @@ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 constexpr int kWarps = 4;                       // consumers
 constexpr int kThreads = (kWarps + 1) * 32;     // and the producer
-constexpr int kTile = 16 * kWarps;              // tokens of a stage, 16 a consumer warp
+// Pieces of 16 tokens that a consumer warp takes from a stage: with rows of 64
+// bytes two at once, so that their chains of dependent products overlap.
+__host__ __device__ constexpr int pieces(int dp) { return dp == 64 ? 2 : 1; }
+__host__ __device__ constexpr int tile_tokens(int dp) { return 16 * kWarps * pieces(dp); }   // tokens of a stage
 constexpr float kGrow = 8.f;           // a maximum may be passed by 2^8 before the sums are rescaled
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kJoin = 4;                     // rows of parts that a joining warp loads at once
@@ -51,11 +54,13 @@ enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
 // four warps' results of a segment.
 template <int DP, int ROWS>
 struct Smem {
-  static constexpr int kStages = DP == 128 ? 3 : 6;
+  static constexpr int kStages = 3;
+  static constexpr int kTile = tile_tokens(DP);
+  static constexpr int kPieces = kTile / 16;
   static constexpr int kSideBytes = kTile * DP;             // K or V of a stage
   static constexpr int kStageBytes = 2 * kSideBytes;
   static constexpr int kOffScales = kStages * kStageBytes;  // [stage][piece]{k scale, v scale}
-  static constexpr int kOffBars = kOffScales + kStages * kWarps * 8;
+  static constexpr int kOffBars = kOffScales + kStages * kPieces * 8;
   static constexpr int kOffMisc = kOffBars + 2 * kStages * 8;
   static constexpr int kOffJoin = kOffMisc + 64;            // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
   static constexpr int kOffO = kOffJoin + 2 * kWarps * ROWS * 4;
@@ -97,8 +102,9 @@ __device__ __forceinline__ int length_of(const Args& a, int r) {
   const int64_t n = a.seq_lens[r], most = a.width << a.lg_block;
   return static_cast<int>(n < 0 ? 0 : (n < most ? n : most));
 }
+template <int TILE>
 __device__ __forceinline__ int tiles_of(const Args& a, int r) {
-  return (length_of(a, r) + kTile - 1) / kTile;
+  return (length_of(a, r) + TILE - 1) / TILE;
 }
 
 __device__ __forceinline__ void mma_16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -154,86 +160,108 @@ struct State {
   float o[N][DP / 16][4];              // dims DP/8 g + 2 t, + 1 (index / 2) of those heads (index % 2)
 };
 
-// One warp's 16 tokens.  k, v: their rows in shared memory, swizzled.
+// One warp's 16 (32) tokens, `left` of them there.  k, v: their rows in shared
+// memory, swizzled; sc: the pieces' scales.
 template <int DP, int ROWS, bool E4M3>
-__device__ __forceinline__ void compute_piece(State<DP, ROWS>& s, const uint8_t* k, const uint8_t* v,
-                                              float ks, float vs, int left, int lane) {
-  constexpr int N = ROWS / 8;
+__device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t* k, const uint8_t* v,
+                                               float2 (&sc)[pieces(DP)], int left, int lane) {
+  constexpr int N = ROWS / 8, P = pieces(DP);
   constexpr int kChunk = DP == 128 ? 8 : 4;      // 16-byte chunks of a row
   const int g = lane >> 2, c = lane & 3;
   // Chunk `at` of a row, in the 128-byte (64-byte) swizzle: XOR of row % 8 ((row / 2) % 4).
   auto place = [&](int row, int at) {
     return row * DP + ((at ^ (DP == 128 ? row & 7 : (row >> 1) & 3)) << 4);
   };
-  float z[N][4];
+  float z[P][N][4];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    z[n][0] = z[n][2] = s.start[n][0];
-    z[n][1] = z[n][3] = s.start[n][1];
-  }
+  for (int x = 0; x < P; ++x) {
 #pragma unroll
-  for (int j = 0; j < DP / 64; ++j) {
-    const int at = kChunk / 4 * c + j;
-    const uint4 x = *reinterpret_cast<const uint4*>(k + place(g, at));
-    const uint4 y = *reinterpret_cast<const uint4*>(k + place(g + 8, at));
-    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+    for (int n = 0; n < N; ++n) {
+      z[x][n][0] = z[x][n][2] = s.start[n][0];
+      z[x][n][1] = z[x][n][3] = s.start[n][1];
+    }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      uint32_t a[4];
-      widen4<E4M3, true>(xs[i], a[0], a[2]);
-      widen4<E4M3, true>(ys[i], a[1], a[3]);
+    for (int j = 0; j < DP / 64; ++j) {
+      const int at = kChunk / 4 * c + j;
+      const uint4 lo = *reinterpret_cast<const uint4*>(k + place(16 * x + g, at));
+      const uint4 hi = *reinterpret_cast<const uint4*>(k + place(16 * x + g + 8, at));
+      const uint32_t ls[4] = {lo.x, lo.y, lo.z, lo.w}, hs[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
-      for (int n = 0; n < N; ++n) mma_16816(z[n], a, s.q[n][4 * j + i][0], s.q[n][4 * j + i][1]);
+      for (int i = 0; i < 4; ++i) {
+        uint32_t a[4];
+        widen4<E4M3, true>(ls[i], a[0], a[2]);
+        widen4<E4M3, true>(hs[i], a[1], a[3]);
+#pragma unroll
+        for (int n = 0; n < N; ++n) mma_16816(z[x][n], a, s.q[n][4 * j + i][0], s.q[n][4 * j + i][1]);
+      }
     }
   }
   // V: tokens 2c, 2c+1, 2c+8, 2c+9, dims DP/8 g ... of each.
-  uint32_t w[4][DP / 32];
+  uint32_t w[P][4][DP / 32];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) {
-    const int row = 2 * c + (t & 1) + (t >> 1) * 8;
-    if (DP == 128) {
-      const uint4 x = *reinterpret_cast<const uint4*>(v + place(row, g));
-      w[t][0] = x.x, w[t][1] = x.y, w[t][DP / 32 - 2] = x.z, w[t][DP / 32 - 1] = x.w;
-    } else {
-      const uint2 x = *reinterpret_cast<const uint2*>(v + place(row, g >> 1) + (g & 1) * 8);
-      w[t][0] = x.x, w[t][1] = x.y;
+  for (int x = 0; x < P; ++x)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = 16 * x + 2 * c + (t & 1) + (t >> 1) * 8;
+      if (DP == 128) {
+        const uint4 y = *reinterpret_cast<const uint4*>(v + place(row, g));
+        w[x][t][0] = y.x, w[x][t][1] = y.y, w[x][t][DP / 32 - 2] = y.z, w[x][t][DP / 32 - 1] = y.w;
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(v + place(row, g >> 1) + (g & 1) * 8);
+        w[x][t][0] = y.x, w[x][t][1] = y.y;
+      }
     }
-  }
-  float top[N][2];
-  bool grow = fabsf(vs) > 16.f * s.unit;
+  bool part = left < 16 * P;
 #pragma unroll
-  for (int n = 0; n < N; ++n)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float r = s.rf[n][h] * ks;
-      z[n][h] *= r;
-      z[n][2 + h] *= r;
-    }
-  if (left < 16) {                       // the last tokens
+  for (int x = 0; x < P; ++x) {
+    const bool out = __float_as_uint(sc[x].x) == kNoBlock;     // a block outside the cache
+    part |= out;
+    if (out) sc[x].y = 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        if (g >= left) z[n][h] = -INFINITY;
-        if (g + 8 >= left) z[n][2 + h] = -INFINITY;
+        const float r = s.rf[n][h] * sc[x].x;
+        z[x][n][h] *= r;
+        z[x][n][2 + h] *= r;
       }
-    // What stands behind them may be NaN in e4m3, and 0 * NaN must not reach the sums.
-    if (E4M3)
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-        if (2 * c + (t & 1) + (t >> 1) * 8 >= left)
-#pragma unroll
-          for (int j = 0; j < DP / 32; ++j) w[t][j] = 0;
   }
+  if (part) {                            // the last tokens, or a block outside the cache
+#pragma unroll
+    for (int x = 0; x < P; ++x) {
+      const int here = __float_as_uint(sc[x].x) == kNoBlock ? 0 : left - 16 * x;
+#pragma unroll
+      for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (g >= here) z[x][n][h] = -INFINITY;
+          if (g + 8 >= here) z[x][n][2 + h] = -INFINITY;
+        }
+      if (here <= 0) sc[x].y = 0.f;
+      // What stands behind them may be NaN in e4m3, and 0 * NaN must not reach the sums.
+      if (E4M3)
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          if (2 * c + (t & 1) + (t >> 1) * 8 >= here)
+#pragma unroll
+            for (int j = 0; j < DP / 32; ++j) w[x][t][j] = 0;
+    }
+  }
+  float top[N][2], most = fabsf(sc[0].y);
+#pragma unroll
+  for (int x = 1; x < P; ++x) most = fmaxf(most, fabsf(sc[x].y));
+  bool grow = most > 16.f * s.unit;
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      top[n][h] = fmaxf(z[n][h], z[n][2 + h]);
+      top[n][h] = fmaxf(z[0][n][h], z[0][n][2 + h]);
+#pragma unroll
+      for (int x = 1; x < P; ++x) top[n][h] = fmaxf(top[n][h], fmaxf(z[x][n][h], z[x][n][2 + h]));
       grow |= top[n][h] > s.m[n][h] + kGrow;
     }
   if (__any_sync(0xffffffffu, grow)) {
-    const float unit = fmaxf(s.unit, fabsf(vs));
+    const float unit = fmaxf(s.unit, most);
     const float ratio = unit > 0.f ? s.unit / unit : 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n)
@@ -255,43 +283,43 @@ __device__ __forceinline__ void compute_piece(State<DP, ROWS>& s, const uint8_t*
     s.unit = unit;
     s.per = unit > 0.f ? 1.f / unit : 0.f;
   }
-  const float weight = vs * s.per;
-  uint32_t p[N][2];
+  uint32_t p[P][N][2];
 #pragma unroll
-  for (int n = 0; n < N; ++n) {
-    float e[4];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const float m = s.m[n][h] == -INFINITY ? 0.f : s.m[n][h];
-      e[h] = exp2_fast(z[n][h] - m);
-      e[2 + h] = exp2_fast(z[n][2 + h] - m);
-      s.l[n][h] += e[h] + e[2 + h];
-    }
-#pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      const __half2 hv = __floats2half2_rn(e[2 * t] * weight, e[2 * t + 1] * weight);
-      p[n][t] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
-    }
-  }
-#pragma unroll
-  for (int j = 0; j < DP / 32; ++j) {
-    uint32_t a[2][4];
-    {
-      const uint32_t x = __byte_perm(w[0][j], w[1][j], 0x5140), y = __byte_perm(w[0][j], w[1][j], 0x7362);
-      widen4<E4M3, false>(x, a[0][0], a[0][1]);
-      widen4<E4M3, false>(y, a[1][0], a[1][1]);
-    }
-    {
-      const uint32_t x = __byte_perm(w[2][j], w[3][j], 0x5140), y = __byte_perm(w[2][j], w[3][j], 0x7362);
-      widen4<E4M3, false>(x, a[0][2], a[0][3]);
-      widen4<E4M3, false>(y, a[1][2], a[1][3]);
-    }
+  for (int x = 0; x < P; ++x) {
+    const float weight = sc[x].y * s.per;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      mma_16816(s.o[n][2 * j], a[0], p[n][0], p[n][1]);
-      mma_16816(s.o[n][2 * j + 1], a[1], p[n][0], p[n][1]);
+      float e[4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float m = s.m[n][h] == -INFINITY ? 0.f : s.m[n][h];
+        e[h] = exp2_fast(z[x][n][h] - m);
+        e[2 + h] = exp2_fast(z[x][n][2 + h] - m);
+        s.l[n][h] += e[h] + e[2 + h];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const __half2 hv = __floats2half2_rn(e[2 * t] * weight, e[2 * t + 1] * weight);
+        p[x][n][t] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
+      }
     }
   }
+#pragma unroll
+  for (int x = 0; x < P; ++x)
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j) {
+      const uint32_t(&u)[4][DP / 32] = w[x];
+      uint32_t a[2][4];
+      widen4<E4M3, false>(__byte_perm(u[0][j], u[1][j], 0x5140), a[0][0], a[0][1]);
+      widen4<E4M3, false>(__byte_perm(u[0][j], u[1][j], 0x7362), a[1][0], a[1][1]);
+      widen4<E4M3, false>(__byte_perm(u[2][j], u[3][j], 0x5140), a[0][2], a[0][3]);
+      widen4<E4M3, false>(__byte_perm(u[2][j], u[3][j], 0x7362), a[1][2], a[1][3]);
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        mma_16816(s.o[n][2 * j], a[0], p[x][n][0], p[x][n][1]);
+        mma_16816(s.o[n][2 * j + 1], a[1], p[x][n][0], p[x][n][1]);
+      }
+    }
 }
 
 template <int DP, int ROWS, bool E4M3>
@@ -361,13 +389,14 @@ __device__ __forceinline__ void store_out(const Args& a, int64_t at, float v) {
 // Tiles before each request: every thread sums a run of requests, the runs'
 // sums are scanned.  Returns the total; *run is the sum before this thread's
 // run, *lo and *hi the run.
+template <int TILE>
 __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo, int* hi, int* run) {
   const int per = (a.requests + kThreads - 1) / kThreads;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   *lo = min(a.requests, static_cast<int>(threadIdx.x) * per);
   *hi = min(a.requests, *lo + per);
   int mine = 0;
-  for (int r = *lo; r < *hi; ++r) mine += tiles_of(a, r);
+  for (int r = *lo; r < *hi; ++r) mine += tiles_of<TILE>(a, r);
   int incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -388,6 +417,7 @@ __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo,
 
 // The segments of a CTA's range of tiles, in order: tiles t0 .. t1 of one
 // request and (virtual) head.
+template <int TILE>
 struct Segments {
   int64_t u, end;
   int r, before;          // request, tiles before it
@@ -397,7 +427,7 @@ struct Segments {
     if (u >= end) return false;
     while (true) {
       len = length_of(a, r);
-      tiles = (len + kTile - 1) / kTile;
+      tiles = (len + TILE - 1) / TILE;
       if (u < static_cast<int64_t>(before + tiles) * heads) break;
       before += tiles;
       ++r;
@@ -446,10 +476,9 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     ptx::fence_mbar_init();
   }
 
-  ptx::griddep_wait();
   int lo, hi, run;
-  const int total = scan_tiles(a, warp_sum, &lo, &hi, &run);
-  Segments seg;
+  const int total = scan_tiles<L::kTile>(a, warp_sum, &lo, &hi, &run);
+  Segments<L::kTile> seg;
   seg.heads = a.kv_heads * a.row_groups;
   const int64_t units = static_cast<int64_t>(total) * seg.heads;
   const int64_t share = (units + a.grid - 1) / a.grid;
@@ -459,7 +488,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     int p = run;
     for (int r = lo; r < hi; ++r) {
       a.prefix[r] = p;
-      p += tiles_of(a, r);
+      p += tiles_of<L::kTile>(a, r);
     }
     if (tid == 0) a.prefix[a.requests] = total;
   }
@@ -467,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
   {
     int p = run;
     for (int r = lo; r < hi; ++r) {
-      const int t = tiles_of(a, r);
+      const int t = tiles_of<L::kTile>(a, r);
       if (seg.u >= static_cast<int64_t>(p) * seg.heads &&
           seg.u < static_cast<int64_t>(p + t) * seg.heads) {
         start[0] = r;
@@ -490,7 +519,8 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     bool ok = true;
     int had = -1;                        // request and first tile of the ids in `id`
     int had_tile = 0, id = -1;
-    const int boxes = kTile / a.box_rows;        // of a stage
+    const int boxes = L::kTile / a.box_rows;     // of a stage
+    constexpr int kBatch = 32 / L::kPieces;      // stages whose blocks the lanes hold
     const int box_pieces = a.box_rows / 16;
     const int box_bytes = a.box_rows * DP;
     while (ok && seg.next(a)) {
@@ -499,12 +529,12 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
       float ks = 0.f, vs = 0.f;
       for (int t = seg.t0; t < seg.t1 && ok; ++t) {
         const int slot = n % L::kStages;
-        if (t == seg.t0 || t - had_tile >= 8) {
-          // Eight stages' blocks and scales at a time, one 16-token piece a lane.
-          if (had != seg.r || t < had_tile || t - had_tile >= 8) {
+        if (t == seg.t0 || t - had_tile >= kBatch) {
+          // Several stages' blocks and scales at a time, one 16-token piece a lane.
+          if (had != seg.r || t < had_tile || t - had_tile >= kBatch) {
             had = seg.r;
             had_tile = t;
-            const int64_t token = static_cast<int64_t>(t) * kTile + 16 * lane;
+            const int64_t token = static_cast<int64_t>(t) * L::kTile + 16 * lane;
             id = token < seg.len ? __ldg(row + (token >> a.lg_block)) : -1;
             if (static_cast<uint32_t>(id) >= a.num_blocks) id = -1;
           }
@@ -519,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
           ok = false;
           break;
         }
-        const int first = (t - had_tile) * kWarps;       // lane of the stage's first piece
+        const int first = (t - had_tile) * L::kPieces;   // lane of the stage's first piece
         const int box_id = __shfl_sync(0xffffffffu, id, (first + lane * box_pieces) & 31);
         const bool load = lane < boxes && box_id >= 0;
         const unsigned loads = __ballot_sync(0xffffffffu, load);
@@ -527,15 +557,15 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
         __syncwarp();
         if (load) {
           uint8_t* to = smem + slot * L::kStageBytes + lane * box_bytes;
-          const int off = (t * kTile + lane * a.box_rows) & ((1 << a.lg_block) - 1);
+          const int off = (t * L::kTile + lane * a.box_rows) & ((1 << a.lg_block) - 1);
           const int y = ((box_id * a.kv_heads + head) << a.lg_block) + off;
           ptx::tma_load_2d(to, &map_k, &full[slot], 0, y);
           ptx::tma_load_2d(to + L::kSideBytes, &map_v, &full[slot], 0, y);
         }
         // The scales, which may still be on their way, complete the stage.
-        if (lane >= first && lane < first + kWarps)
+        if (lane >= first && lane < first + L::kPieces)
           // A block outside the cache leaves its tokens out.
-          scales[slot * kWarps + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
+          scales[slot * L::kPieces + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&full[slot]);
         __syncwarp();
@@ -572,11 +602,14 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
         if (lane == 0) fail(a.err, abort_flag, kErrFull);
         break;
       }
-      const int left = seg.len - t * kTile - warp * 16;
-      const float2 sc = scales[slot * kWarps + warp];
-      if (left > 0 && __float_as_uint(sc.x) != kNoBlock) {
-        const uint8_t* k = smem + slot * L::kStageBytes + warp * 16 * DP;
-        compute_piece<DP, ROWS, E4M3>(s, k, k + L::kSideBytes, sc.x, sc.y, left, lane);
+      constexpr int P = pieces(DP);
+      const int left = seg.len - t * L::kTile - warp * 16 * P;
+      float2 sc[P];
+#pragma unroll
+      for (int x = 0; x < P; ++x) sc[x] = scales[slot * L::kPieces + warp * P + x];
+      if (left > 0) {
+        const uint8_t* k = smem + slot * L::kStageBytes + warp * 16 * P * DP;
+        compute_pieces<DP, ROWS, E4M3>(s, k, k + L::kSideBytes, sc, left, lane);
       }
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&empty[slot]);
@@ -642,7 +675,6 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
 template <int DP, int ROWS>
 __global__ void cache_join_kernel(const Args a) {
   extern __shared__ float sm[];          // [warps][DP + 1]
-  ptx::griddep_launch_dependents();
   ptx::griddep_wait();
   const int heads = a.kv_heads * a.row_groups;
   const int j = blockIdx.x % (a.kv_heads * a.group), r = blockIdx.x / (a.kv_heads * a.group);
@@ -743,7 +775,7 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   w.dp = d->dim <= 64 ? 64 : 128;
   w.row_groups = static_cast<int>(cdiv(group, w.rows));
   const int64_t most = d->requests * d->kv_heads * w.row_groups *
-                       std::max<int64_t>(cdiv(d->table_width * d->block_size, kTile), 1);
+                       std::max<int64_t>(cdiv(d->table_width * d->block_size, tile_tokens(w.dp)), 1);
   w.grid = static_cast<int>(std::min<int64_t>(
       std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * (w.rows == 8 ? Smem<128, 8>::kCtas : Smem<128, 16>::kCtas)));
   auto pad = [](int64_t n) { return cdiv(n, 256) * 256; };
@@ -777,8 +809,9 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
       return B2G_ERR_LAUNCH;
     configured = dev;
   }
-  // Both kernels may be set up while the one before them on the stream still runs; they wait for it
-  // before they touch memory.
+  // The join may be set up while the kernel before it runs, and waits for it before it reads.  (Not
+  // so the attention itself: started among the join's CTAs of the call before, its own can end up
+  // unevenly spread, 16 requests of 20000 tokens then took 152 us for 111.)
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -788,12 +821,13 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
-  cfg.numAttrs = b2g::pdl_enabled() ? 1 : 0;
+  cfg.numAttrs = 0;
   if (cudaLaunchKernelEx(&cfg, cache_attention_kernel<DP, ROWS, E4M3>, mk, mv, a) != cudaSuccess)
     return B2G_ERR_LAUNCH;
   const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
   // Parts of a head, were all lengths alike.
   const int warps = a.grid > 16 * a.requests * a.kv_heads * a.row_groups ? 16 : 4;
+  cfg.numAttrs = b2g::pdl_enabled() ? 1 : 0;
   cfg.gridDim = dim3(static_cast<unsigned>(a.requests * heads), 1, 1);
   cfg.blockDim = dim3(warps * 32, 1, 1);
   cfg.dynamicSmemBytes = warps * (DP + 1) * sizeof(float);
@@ -858,7 +892,7 @@ extern "C" int b2g_cache_attention(const b2g_cache_attention_desc* d, b2g_stream
   a.grid = w.grid;
   a.wait_limit_ns = b2g::current_wait_limit_ns();
   a.err = dev.error_word;
-  a.box_rows = static_cast<int>(std::min<int64_t>(d->block_size, kTile));
+  a.box_rows = static_cast<int>(std::min<int64_t>(d->block_size, tile_tokens(w.dp)));
   CUtensorMap mk = {}, mv = {};
   const int64_t cache_rows = d->num_blocks * d->kv_heads * d->block_size;
   if (d->num_blocks > 0 && (!make_map(&mk, d->k_cache, d->dim, cache_rows, w.dp, a.box_rows) ||

@@ -33,7 +33,7 @@ int log2_of(int64_t x) {
 // block writes the table entry.  No CTA reads what another writes, so one
 // launch does it all.  Bound by latency: launch, one load of the lengths,
 // one dependent load of the block, one store.
-constexpr int kTableThreads = 512;
+constexpr int kTableThreadsMost = 1024;
 
 struct TableArgs {
   const int32_t* context_lens;
@@ -57,21 +57,24 @@ __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int lg, int64_t wid
   return n < width ? n : width;
 }
 
-__global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const TableArgs a) {
+__global__ void __launch_bounds__(kTableThreadsMost) block_tables_kernel(const TableArgs a) {
   extern __shared__ int smem[];
   int* cu = smem;                        // requests + 1: new tokens before each request
-  int* first = smem + a.requests + 1;    // new blocks before each request
-  __shared__ unsigned long long warp_sum[kTableThreads / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int* first = cu + a.requests + 1;      // new blocks before each request
+  int* had = first + a.requests;         // tokens that it holds
+  __shared__ unsigned long long warp_sum[kTableThreadsMost / 32];
+  const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t count = min(static_cast<int64_t>(*a.free_count), a.free_capacity);
   // Scan of (tokens, blocks) as the halves of one 64-bit word.
   unsigned long long carry = 0;
-  for (int base = 0; base < a.requests; base += kTableThreads) {
+  for (int base = 0; base < a.requests; base += threads) {
     const int r = base + tid;
     unsigned long long v = 0;
     if (r < a.requests) {
       const int64_t ctx = max(a.context_lens[r], 0), add = max(a.new_lens[r], 0);
       const int64_t need =
           blocks_of(ctx + add, a.lg_block, a.width) - blocks_of(ctx, a.lg_block, a.width);
+      had[r] = static_cast<int>(ctx);
       v = static_cast<unsigned long long>(need) << 32 | static_cast<unsigned long long>(add);
       if (blockIdx.x == 0) a.seq_lens[r] = static_cast<int32_t>(ctx + add);
     }
@@ -84,8 +87,7 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const Table
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
     unsigned long long before = carry;
-#pragma unroll
-    for (int w = 0; w < kTableThreads / 32; ++w) {
+    for (int w = 0; w < threads / 32; ++w) {
       const unsigned long long s = warp_sum[w];
       if (w < warp) before += s;
       carry += s;
@@ -107,10 +109,9 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const Table
     }
   }
   __syncthreads();
-  const int64_t count = min(static_cast<int64_t>(*a.free_count), a.free_capacity);
   const int64_t end = max(sum, a.total);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * kTableThreads;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * kTableThreads + tid; t < end; t += step) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * threads;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * threads + tid; t < end; t += step) {
     int64_t slot = -1;
     if (t < sum) {
       // The last request that begins at or before t.  One token each is the
@@ -125,7 +126,7 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const Table
           else hi = mid;
         }
       }
-      const int64_t ctx = max(a.context_lens[lo], 0);
+      const int64_t ctx = had[lo];
       const int64_t pos = ctx + (t - cu[lo]);
       const int64_t j = pos >> a.lg_block;
       const int off = static_cast<int>(pos & ((int64_t{1} << a.lg_block) - 1));
@@ -156,8 +157,6 @@ __global__ void __launch_bounds__(kTableThreads) block_tables_kernel(const Table
 // does not depend on the order.  Bound by memory: 2 bytes read and 1 written
 // a value.
 constexpr int kAppendWarps = 8;
-constexpr int kHold = 8;   // 16-byte vectors of a group that a lane keeps between the two passes
-
 struct AppendArgs {
   const uint16_t* x[2];          // keys, values
   int64_t token_stride[2], head_stride[2];
@@ -204,8 +203,10 @@ __device__ __forceinline__ float decode1(uint32_t byte) {
   return static_cast<float>(static_cast<int8_t>(byte));
 }
 
-template <bool BF16, bool E4M3>
-__global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const AppendArgs a) {
+// HOLD: 16-byte vectors of a group that a lane keeps between the two passes.
+template <bool BF16, bool E4M3, int HOLD>
+__global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
+    cache_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t item = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
   if (item >= a.items) return;
@@ -219,14 +220,15 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
   constexpr uint32_t kInf = BF16 ? 0x7f80u : 0x7c00u;
   constexpr float kInvQmax = E4M3 ? 1.f / 448.f : 1.f / 127.f;
 
-  // Groups that begin in this chunk.
-  int64_t slot = -1;
+  // Groups that begin in this chunk, and the slots of 64 tokens from its first on.
+  int64_t slot = -1, later = -1;
   bool lead = false;
-  if (lane < a.chunk && t0 + lane < a.tokens) {
+  if (t0 + lane < a.tokens) {
     slot = a.slots[t0 + lane];
     const int64_t prev = t0 + lane > 0 ? a.slots[t0 + lane - 1] : -2;
-    lead = slot >= 0 && slot < a.limit && (prev != slot - 1 || (slot & (bs - 1)) == 0);
+    lead = lane < a.chunk && slot >= 0 && slot < a.limit && (prev != slot - 1 || (slot & (bs - 1)) == 0);
   }
+  if (t0 + 32 + lane < a.tokens) later = a.slots[t0 + 32 + lane];
   unsigned leads = __ballot_sync(0xffffffffu, lead);
   const int row = lane / a.lanes_row, col = lane % a.lanes_row;
   const bool used = row < a.rows_warp;
@@ -237,22 +239,26 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
     const int64_t t = t0 + src;
     const int fill = static_cast<int>(s0 & (bs - 1));
     const int64_t block = s0 >> a.lg_block;
-    // The group's length.
-    int n = 1;
-    while (n < bs - fill) {
-      const int i = n + lane;
-      const bool same = i < bs - fill && t + i < a.tokens && a.slots[t + i] == s0 + i;
-      const unsigned m = __ballot_sync(0xffffffffu, same);
-      n += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
-      if (m != 0xffffffffu) break;
-    }
+    // The group's length: consecutive slots, first among the 64 at hand.
+    const uint64_t run =
+        (static_cast<uint64_t>(__ballot_sync(0xffffffffu, later == s0 + 32 + lane - src)) << 32 |
+         __ballot_sync(0xffffffffu, slot == s0 + lane - src)) >> src;
+    int n = min(bs - fill, ~run ? __ffsll(static_cast<long long>(~run)) - 1 : 64);
+    if (n == 64 - src)
+      while (n < bs - fill) {
+        const int i = n + lane;
+        const bool same = i < bs - fill && t + i < a.tokens && a.slots[t + i] == s0 + i;
+        const unsigned m = __ballot_sync(0xffffffffu, same);
+        n += m == 0xffffffffu ? 32 : __ffs(~m) - 1;
+        if (m != 0xffffffffu) break;
+      }
     const uint16_t* xr = x + t * ts + col * 8;
-    uint4 held[kHold];
+    uint4 held[HOLD];
     uint32_t most = 0;           // largest |x| bits, two halves
-    const int span = kHold * a.rows_warp;
+    const int span = HOLD * a.rows_warp;
     auto load = [&](int base) {
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
+      for (int i = 0; i < HOLD; ++i) {
         const int rr = base + i * a.rows_warp + row;
         held[i] = make_uint4(0, 0, 0, 0);
         if (used && rr < n) held[i] = __ldg(reinterpret_cast<const uint4*>(xr + rr * ts));
@@ -261,7 +267,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
     for (int base = 0; base < n; base += span) {
       load(base);
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
+      for (int i = 0; i < HOLD; ++i) {
         const uint32_t w = __vmaxu2(__vmaxu2(held[i].x & 0x7fff7fffu, held[i].y & 0x7fff7fffu),
                                     __vmaxu2(held[i].z & 0x7fff7fffu, held[i].w & 0x7fff7fffu));
         most = __vmaxu2(most, w);
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
       uint32_t m = 0;
       for (int base = 0; base < n; base += span) {
         load(base);
-        for (int i = 0; i < kHold; ++i) {
+        for (int i = 0; i < HOLD; ++i) {
           const uint32_t v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
           for (int j = 0; j < 4; ++j) {
             const uint32_t lo = v[j] & 0x7fffu, hi = (v[j] >> 16) & 0x7fffu;
@@ -311,7 +317,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32) cache_append_kernel(const A
     for (int base = 0; base < n; base += span) {
       if (n > span) load(base);   // else still held (a lane's rows past n hold zeros)
 #pragma unroll
-      for (int i = 0; i < kHold; ++i) {
+      for (int i = 0; i < HOLD; ++i) {
         const int rr = base + i * a.rows_warp + row;
         if (used && rr < n) {
           const float2 p0 = widen<BF16>(held[i].x), p1 = widen<BF16>(held[i].y);
@@ -366,14 +372,16 @@ extern "C" int b2g_block_tables(const int32_t* context_lens, const int32_t* new_
   a.cu = cu_seqlens;
   a.seq_lens = seq_lens;
   a.free_out = free_count_out;
-  const size_t bytes = (2 * requests + 1) * sizeof(int);
+  const size_t bytes = (3 * requests + 1) * sizeof(int);
   if (bytes > 48 * 1024 &&
       cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(bytes)) != cudaSuccess)
     return B2G_ERR_LAUNCH;
+  // One pass of the scan where 1024 threads allow it; a small step starts faster with fewer.
+  const int threads = requests <= 256 ? 256 : kTableThreadsMost;
   const int grid = static_cast<int>(
-      std::min<int64_t>(std::max<int64_t>(cdiv(total_tokens, kTableThreads), 1), dev.num_sms));
-  block_tables_kernel<<<grid, kTableThreads, bytes, static_cast<cudaStream_t>(stream_handle)>>>(a);
+      std::min<int64_t>(std::max<int64_t>(cdiv(total_tokens, threads), 1), dev.num_sms));
+  block_tables_kernel<<<grid, threads, bytes, static_cast<cudaStream_t>(stream_handle)>>>(a);
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }
 
@@ -426,8 +434,14 @@ extern "C" int b2g_cache_append(const b2g_cache_append_desc* d, b2g_stream_t str
   if (grid > 0x7fffffff) return B2G_ERR_UNSUPPORTED;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf = d->dtype == B2G_BF16, e4 = d->codes == B2G_E4M3;
-  auto* kernel = bf ? (e4 ? cache_append_kernel<true, true> : cache_append_kernel<true, false>)
-                    : (e4 ? cache_append_kernel<false, true> : cache_append_kernel<false, false>);
+  // A whole block's rows in registers up to 32 rows of 128 values; more are read twice.
+  const bool wide = d->block_size > 16 && d->tokens > d->block_size;
+  auto pick = [&](auto narrow_kernel, auto wide_kernel) { return wide ? wide_kernel : narrow_kernel; };
+  auto* kernel =
+      bf ? (e4 ? pick(cache_append_kernel<true, true, 8>, cache_append_kernel<true, true, 16>)
+               : pick(cache_append_kernel<true, false, 8>, cache_append_kernel<true, false, 16>))
+         : (e4 ? pick(cache_append_kernel<false, true, 8>, cache_append_kernel<false, true, 16>)
+               : pick(cache_append_kernel<false, false, 8>, cache_append_kernel<false, false, 16>));
   kernel<<<static_cast<unsigned>(grid), kAppendWarps * 32, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }

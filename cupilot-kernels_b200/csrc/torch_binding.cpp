@@ -9,6 +9,7 @@
 // torch::empty (every element is written by the kernel), launches on the
 // current CUDA stream and never synchronises the host.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -483,6 +484,12 @@ int dtype_of(const at::Tensor& t, const char* name) {
   return dt == at::kHalf ? B2G_F16 : B2G_BF16;
 }
 
+// An uninitialised tensor beside `like`, without the dispatcher: a serving
+// step's small calls take a few microseconds in all.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, dt, like.device(), c10::nullopt);
+}
+
 void check_ints(const at::Tensor& t, const char* name, int64_t dims, at::ScalarType dt,
                 const at::Tensor& like) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the same CUDA device");
@@ -535,7 +542,7 @@ Cache check_cache(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& 
   return {dt == at::kChar ? B2G_I8 : B2G_E4M3, kc.size(0), kc.size(1), bs, d};
 }
 
-std::vector<at::Tensor> block_tables(const at::Tensor& context_lens, const at::Tensor& new_lens,
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> block_tables(const at::Tensor& context_lens, const at::Tensor& new_lens,
                                      const at::Tensor& block_table, const at::Tensor& free_blocks,
                                      const at::Tensor& free_count, int64_t total_tokens,
                                      int64_t block_size) {
@@ -559,10 +566,10 @@ std::vector<at::Tensor> block_tables(const at::Tensor& context_lens, const at::T
               "block_size must be a power of two from 16 to 256, got ", block_size);
   TORCH_CHECK(n <= B2G_MAX_TABLE_REQUESTS, "at most ", B2G_MAX_TABLE_REQUESTS, " requests");
   const c10::cuda::CUDAGuard guard(context_lens.device());
-  at::Tensor slots = at::empty({total_tokens}, context_lens.options().dtype(at::kLong));
-  at::Tensor cu = at::empty({n + 1}, context_lens.options());
-  at::Tensor lens = at::empty({n}, context_lens.options());
-  at::Tensor left = at::empty({1}, context_lens.options());
+  at::Tensor slots = fresh({total_tokens}, at::kLong, context_lens);
+  at::Tensor cu = fresh({n + 1}, at::kInt, context_lens);
+  at::Tensor lens = fresh({n}, at::kInt, context_lens);
+  at::Tensor left = fresh({1}, at::kInt, context_lens);
   auto stream = at::cuda::getCurrentCUDAStream(context_lens.device().index());
   check_status(
       b2g_block_tables(context_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n,
@@ -650,9 +657,9 @@ py::object cache_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   TORCH_CHECK(seq_lens.size(0) == n, "seq_lens must have one value for each request");
   d.scale = scale_of(scale);
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor out = fresh(q.sizes(), q.scalar_type(), q);
   at::Tensor lse;
-  if (return_lse) lse = at::empty({n, heads}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = fresh({n, heads}, at::kFloat, q);
   if (out.numel() == 0) return with_lse(out, lse, return_lse);
   const at::Tensor qr = rows_of(q);
   d.codes = c.codes;
@@ -677,7 +684,7 @@ py::object cache_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   d.lse = return_lse ? lse.data_ptr<float>() : nullptr;
   const int64_t ws = b2g_cache_attention_workspace_bytes(&d);
   TORCH_CHECK(ws >= 0, "b2g: cache attention beyond the supported sizes");
-  const at::Tensor wst = at::empty({ws}, q.options().dtype(at::kByte));
+  const at::Tensor wst = fresh({ws}, at::kByte, q);
   d.workspace = wst.data_ptr();
   d.workspace_bytes = ws;
   auto stream = at::cuda::getCurrentCUDAStream(q.device().index());
@@ -716,9 +723,9 @@ py::object prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::
   }
   d.scale = scale_of(scale);
   const c10::cuda::CUDAGuard guard(q.device());
-  at::Tensor out = at::empty(q.sizes(), q.options());
+  at::Tensor out = fresh(q.sizes(), q.scalar_type(), q);
   at::Tensor lse;
-  if (return_lse) lse = at::empty({q.size(0), heads}, q.options().dtype(at::kFloat));
+  if (return_lse) lse = fresh({q.size(0), heads}, at::kFloat, q);
   if (out.numel() == 0) return with_lse(out, lse, return_lse);
   const at::Tensor qr = rows_of(q), kr = rows_of(k), vr = rows_of(v);
   d.causal = causal;

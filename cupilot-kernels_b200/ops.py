@@ -166,8 +166,8 @@ def block_tables(context_lens, new_lens, block_table, free_blocks, free_count, t
     (requests + 1), the lengths after the step, and what is left of the
     stack (below 0: that many blocks were missing).
     """
-    return tuple(_ext.block_tables(context_lens, new_lens, block_table, free_blocks, free_count,
-                                   total_tokens, block_size))
+    return _ext.block_tables(context_lens, new_lens, block_table, free_blocks, free_count,
+                             total_tokens, block_size)
 
 
 def cache_append(k, v, slots, k_cache, v_cache, k_scale, v_scale):
