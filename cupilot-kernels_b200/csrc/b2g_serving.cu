@@ -33,7 +33,6 @@ int log2_of(int64_t x) {
 // block writes the table entry.  No CTA reads what another writes, so one
 // launch does it all.  Bound by latency: launch, one load of the lengths,
 // one dependent load of the block, one store.
-constexpr int kTableThreadsMost = 1024;
 
 struct TableArgs {
   const int32_t* context_lens;
@@ -57,21 +56,26 @@ __device__ __forceinline__ int64_t blocks_of(int64_t tokens, int lg, int64_t wid
   return n < width ? n : width;
 }
 
-__global__ void __launch_bounds__(kTableThreadsMost) block_tables_kernel(const TableArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) block_tables_kernel(const TableArgs a) {
   extern __shared__ int smem[];
   int* cu = smem;                        // requests + 1: new tokens before each request
   int* first = cu + a.requests + 1;      // new blocks before each request
   int* had = first + a.requests;         // tokens that it holds
-  __shared__ unsigned long long warp_sum[kTableThreadsMost / 32];
-  const int threads = blockDim.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ unsigned long long warp_sum[THREADS / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t count = min(static_cast<int64_t>(*a.free_count), a.free_capacity);
   // Scan of (tokens, blocks) as the halves of one 64-bit word.
   unsigned long long carry = 0;
-  for (int base = 0; base < a.requests; base += threads) {
+  int next_ctx = 0, next_add = 0;        // of the next round, on their way during this one
+  if (tid < a.requests) next_ctx = a.context_lens[tid], next_add = a.new_lens[tid];
+  for (int base = 0; base < a.requests; base += THREADS) {
     const int r = base + tid;
     unsigned long long v = 0;
+    const int64_t ctx = max(next_ctx, 0), add = max(next_add, 0);
+    if (r + THREADS < a.requests)
+      next_ctx = a.context_lens[r + THREADS], next_add = a.new_lens[r + THREADS];
     if (r < a.requests) {
-      const int64_t ctx = max(a.context_lens[r], 0), add = max(a.new_lens[r], 0);
       const int64_t need =
           blocks_of(ctx + add, a.lg_block, a.width) - blocks_of(ctx, a.lg_block, a.width);
       had[r] = static_cast<int>(ctx);
@@ -87,7 +91,8 @@ __global__ void __launch_bounds__(kTableThreadsMost) block_tables_kernel(const T
     if (lane == 31) warp_sum[warp] = incl;
     __syncthreads();
     unsigned long long before = carry;
-    for (int w = 0; w < threads / 32; ++w) {
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
       const unsigned long long s = warp_sum[w];
       if (w < warp) before += s;
       carry += s;
@@ -110,8 +115,8 @@ __global__ void __launch_bounds__(kTableThreadsMost) block_tables_kernel(const T
   }
   __syncthreads();
   const int64_t end = max(sum, a.total);
-  const int64_t step = static_cast<int64_t>(gridDim.x) * threads;
-  for (int64_t t = static_cast<int64_t>(blockIdx.x) * threads + tid; t < end; t += step) {
+  const int64_t step = static_cast<int64_t>(gridDim.x) * THREADS;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * THREADS + tid; t < end; t += step) {
     int64_t slot = -1;
     if (t < sum) {
       // The last request that begins at or before t.  One token each is the
@@ -149,8 +154,8 @@ __global__ void __launch_bounds__(kTableThreadsMost) block_tables_kernel(const T
 }
 
 // ------------------------------------------------------------ cache write
-// A warp takes a chunk of consecutive tokens for one head of the keys or the
-// values and does the groups that begin in it, one after another: the largest
+// W warps take a chunk of consecutive tokens for one head of the keys or the
+// values and do the groups that begin in it, one after another: the largest
 // |x| of the group, the block's new scale, the old codes moved to it where it
 // grew, the new codes.  The group's owner is the only one that touches the
 // block's codes and scale of that head, so nothing is atomic and the result
@@ -203,13 +208,27 @@ __device__ __forceinline__ float decode1(uint32_t byte) {
   return static_cast<float>(static_cast<int8_t>(byte));
 }
 
-// HOLD: 16-byte vectors of a group that a lane keeps between the two passes.
-template <bool BF16, bool E4M3, int HOLD>
-__global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
+template <bool BF16, bool E4M3, int W>
+__global__ void __launch_bounds__(kAppendWarps * 32, 3)
     cache_append_kernel(const AppendArgs a) {
+  constexpr int kHold = 8;                 // 16-byte vectors that a lane keeps between the passes
+  __shared__ uint32_t tops[kAppendWarps];
   const int lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * kAppendWarps + (threadIdx.x >> 5);
+  const int warp = threadIdx.x >> 5, sub = warp % W;
+  const int64_t item = static_cast<int64_t>(blockIdx.x) * (kAppendWarps / W) + warp / W;
   if (item >= a.items) return;
+  // The largest of the item's warps.
+  auto largest = [&](uint32_t x) {
+    x = __reduce_max_sync(0xffffffffu, x);
+    if (W == 1) return x;
+    auto meet = [&]() { asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / W), "n"(W * 32) : "memory"); };
+    if (lane == 0) tops[warp] = x;
+    meet();
+#pragma unroll
+    for (int w = 0; w < W; ++w) x = max(x, tops[warp / W * W + w]);
+    meet();                                // read before it is written again
+    return x;
+  };
   const int both = 2 * a.heads;
   const int64_t t0 = item / both * a.chunk;
   const int hk = static_cast<int>(item % both);
@@ -253,13 +272,13 @@ __global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
         if (m != 0xffffffffu) break;
       }
     const uint16_t* xr = x + t * ts + col * 8;
-    uint4 held[HOLD];
+    uint4 held[kHold];
     uint32_t most = 0;           // largest |x| bits, two halves
-    const int span = HOLD * a.rows_warp;
+    const int step = W * a.rows_warp, span = kHold * step;
     auto load = [&](int base) {
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i) {
-        const int rr = base + i * a.rows_warp + row;
+      for (int i = 0; i < kHold; ++i) {
+        const int rr = base + i * step + sub * a.rows_warp + row;
         held[i] = make_uint4(0, 0, 0, 0);
         if (used && rr < n) held[i] = __ldg(reinterpret_cast<const uint4*>(xr + rr * ts));
       }
@@ -267,19 +286,19 @@ __global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
     for (int base = 0; base < n; base += span) {
       load(base);
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i) {
+      for (int i = 0; i < kHold; ++i) {
         const uint32_t w = __vmaxu2(__vmaxu2(held[i].x & 0x7fff7fffu, held[i].y & 0x7fff7fffu),
                                     __vmaxu2(held[i].z & 0x7fff7fffu, held[i].w & 0x7fff7fffu));
         most = __vmaxu2(most, w);
       }
     }
-    uint32_t top = __reduce_max_sync(0xffffffffu, max(most & 0xffffu, most >> 16));
+    uint32_t top = largest(max(most & 0xffffu, most >> 16));
     const bool any = top >= kInf;          // an infinity or NaN: look again without those
     if (any) {
       uint32_t m = 0;
       for (int base = 0; base < n; base += span) {
         load(base);
-        for (int i = 0; i < HOLD; ++i) {
+        for (int i = 0; i < kHold; ++i) {
           const uint32_t v[4] = {held[i].x, held[i].y, held[i].z, held[i].w};
           for (int j = 0; j < 4; ++j) {
             const uint32_t lo = v[j] & 0x7fffu, hi = (v[j] >> 16) & 0x7fffu;
@@ -288,20 +307,21 @@ __global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
           }
         }
       }
-      top = __reduce_max_sync(0xffffffffu, m);
+      top = largest(m);
     }
     const float amax = widen<BF16>(top).x;
     float* sp = a.scale[kv] + block * a.heads + head;
     const float old = fill > 0 ? *sp : 0.f;
+    if (W > 1 && fill > 0) largest(0);       // every warp has read the scale
     const float now = fmaxf(old, __fmul_rn(amax, kInvQmax));
     // Without a finite value but 0 the steps are 0; 1 then, so that an infinity stays one.
     const float steps = now > 0.f ? fminf(__fdiv_rn(1.f, now), FLT_MAX) : (any ? 1.f : 0.f);
     __syncwarp();
-    if (lane == 0) *sp = now;
+    if (lane == 0 && sub == 0) *sp = now;
     uint8_t* cp = a.cache[kv] + ((block * a.heads + head) << a.lg_block) * a.dim + col * 8;
     if (fill > 0 && now > old) {
       const float ratio = __fdiv_rn(old, now);
-      for (int rr = row; rr < fill && used; rr += a.rows_warp) {
+      for (int rr = sub * a.rows_warp + row; rr < fill && used; rr += step) {
         uint2* p = reinterpret_cast<uint2*>(cp + rr * a.dim);
         const uint2 w = *p;
         float f[8];
@@ -317,8 +337,8 @@ __global__ void __launch_bounds__(kAppendWarps * 32, HOLD == 8 ? 3 : 2)
     for (int base = 0; base < n; base += span) {
       if (n > span) load(base);   // else still held (a lane's rows past n hold zeros)
 #pragma unroll
-      for (int i = 0; i < HOLD; ++i) {
-        const int rr = base + i * a.rows_warp + row;
+      for (int i = 0; i < kHold; ++i) {
+        const int rr = base + i * step + sub * a.rows_warp + row;
         if (used && rr < n) {
           const float2 p0 = widen<BF16>(held[i].x), p1 = widen<BF16>(held[i].y);
           const float2 p2 = widen<BF16>(held[i].z), p3 = widen<BF16>(held[i].w);
@@ -373,15 +393,18 @@ extern "C" int b2g_block_tables(const int32_t* context_lens, const int32_t* new_
   a.seq_lens = seq_lens;
   a.free_out = free_count_out;
   const size_t bytes = (3 * requests + 1) * sizeof(int);
+  // Fewer threads start a small step sooner (8 requests: 2.4 us for 2.9), more scan a large one in
+  // fewer rounds.
+  const bool small = requests <= 256;
+  const int threads = small ? 256 : 512;
+  auto* kernel = small ? block_tables_kernel<256> : block_tables_kernel<512>;
   if (bytes > 48 * 1024 &&
-      cudaFuncSetAttribute(block_tables_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                            static_cast<int>(bytes)) != cudaSuccess)
     return B2G_ERR_LAUNCH;
-  // One pass of the scan where 1024 threads allow it; a small step starts faster with fewer.
-  const int threads = requests <= 256 ? 256 : kTableThreadsMost;
   const int grid = static_cast<int>(
       std::min<int64_t>(std::max<int64_t>(cdiv(total_tokens, threads), 1), dev.num_sms));
-  block_tables_kernel<<<grid, threads, bytes, static_cast<cudaStream_t>(stream_handle)>>>(a);
+  kernel<<<grid, threads, bytes, static_cast<cudaStream_t>(stream_handle)>>>(a);
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }
 
@@ -430,18 +453,20 @@ extern "C" int b2g_cache_append(const b2g_cache_append_desc* d, b2g_stream_t str
       std::max<int64_t>(d->tokens * per_token / (16ll * dev.num_sms), 1),
       std::min<int64_t>(d->block_size, 32)));
   a.items = cdiv(d->tokens, a.chunk) * per_token;
-  const int64_t grid = cdiv(a.items, kAppendWarps);
+  // Warps to an item: one, but for whole large blocks, of which there are too few to fill the GPU
+  // (18000 tokens in blocks of 16, 32, 64: 20, 22, 22 us with one warp, 20, 25, 30 with more; of
+  // 128: 31 and 29).
+  const int w = d->block_size < 128 || d->tokens <= d->block_size ? 1 : 4;
+  const int64_t grid = cdiv(a.items, kAppendWarps / w);
   if (grid > 0x7fffffff) return B2G_ERR_UNSUPPORTED;
   cudaStream_t stream = static_cast<cudaStream_t>(stream_handle);
   const bool bf = d->dtype == B2G_BF16, e4 = d->codes == B2G_E4M3;
-  // A whole block's rows in registers up to 32 rows of 128 values; more are read twice.
-  const bool wide = d->block_size > 16 && d->tokens > d->block_size;
-  auto pick = [&](auto narrow_kernel, auto wide_kernel) { return wide ? wide_kernel : narrow_kernel; };
+  auto pick = [&](auto* one, auto* four) { return w == 1 ? one : four; };
   auto* kernel =
-      bf ? (e4 ? pick(cache_append_kernel<true, true, 8>, cache_append_kernel<true, true, 16>)
-               : pick(cache_append_kernel<true, false, 8>, cache_append_kernel<true, false, 16>))
-         : (e4 ? pick(cache_append_kernel<false, true, 8>, cache_append_kernel<false, true, 16>)
-               : pick(cache_append_kernel<false, false, 8>, cache_append_kernel<false, false, 16>));
+      bf ? (e4 ? pick(cache_append_kernel<true, true, 1>, cache_append_kernel<true, true, 4>)
+               : pick(cache_append_kernel<true, false, 1>, cache_append_kernel<true, false, 4>))
+         : (e4 ? pick(cache_append_kernel<false, true, 1>, cache_append_kernel<false, true, 4>)
+               : pick(cache_append_kernel<false, false, 1>, cache_append_kernel<false, false, 4>));
   kernel<<<static_cast<unsigned>(grid), kAppendWarps * 32, 0, stream>>>(a);
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }
