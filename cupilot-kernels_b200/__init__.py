@@ -6,6 +6,10 @@ each operator keeps the reference's Torch C++-extension entry point
 Part-3 name, see `ops`), implemented by hand-written tcgen05/TMA kernels in
 `libb2g_sm100.so` behind the C ABI in `include/b2g_gemm.h`.
 
+`serving` holds a paged 8-bit key/value cache over the serving operators
+(block tables, cache write, cache attention, prompt attention; the C ABI in
+`include/b2g_serving.h`).
+
 There is no CPU or library fallback: importing `ops` without the built
 extension raises ImportError.
 """
@@ -34,7 +38,7 @@ def native():
 
 
 def __getattr__(name):
-    if name in ("ops", "partition", "capi"):
+    if name in ("ops", "partition", "capi", "serving"):
         import importlib
 
         return importlib.import_module(f"{__name__}.{name}")

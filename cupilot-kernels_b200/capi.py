@@ -1,4 +1,4 @@
-"""ctypes binding of the C ABI in include/b2g_gemm.h.
+"""ctypes binding of the C ABI in include/b2g_gemm.h and include/b2g_serving.h.
 
 This is the same binding a non-Torch host would write (cgo / JNI / N-API
 stubs look alike): plain structs, pointers and sizes.  Device pointers and
@@ -34,6 +34,52 @@ class GemmDesc(C.Structure):
         ("b", C.c_void_p), ("ldb", C.c_int64), ("stride_b", C.c_int64), ("trans_b", C.c_int32),
         ("c", C.c_void_p), ("ldc", C.c_int64), ("stride_c", C.c_int64),
         ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+# include/b2g_serving.h
+F16, BF16 = 0, 1                # b2g_dtype
+I8, E4M3 = 0, 1                 # b2g_codes
+MAX_TABLE_REQUESTS = 16384
+
+
+class CacheAppendDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("codes", C.c_int32),
+        ("tokens", C.c_int64), ("kv_heads", C.c_int64), ("dim", C.c_int64),
+        ("num_blocks", C.c_int64), ("block_size", C.c_int64),
+        ("k", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v", C.c_void_p), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("slots", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+    ]
+
+
+class CacheAttentionDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("codes", C.c_int32),
+        ("requests", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
+        ("dim", C.c_int64), ("num_blocks", C.c_int64), ("block_size", C.c_int64),
+        ("q", C.c_void_p), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+        ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+        ("block_table", C.c_void_p), ("table_width", C.c_int64), ("table_ld", C.c_int64),
+        ("seq_lens", C.c_void_p), ("scale", C.c_float),
+        ("out", C.c_void_p), ("lse", C.c_void_p),
+        ("workspace", C.c_void_p), ("workspace_bytes", C.c_int64),
+    ]
+
+
+class PromptAttentionDesc(C.Structure):
+    _fields_ = [
+        ("dtype", C.c_int32), ("causal", C.c_int32),
+        ("tokens", C.c_int64), ("tokens_k", C.c_int64), ("sequences", C.c_int64),
+        ("heads", C.c_int64), ("kv_heads", C.c_int64), ("dim", C.c_int64),
+        ("q", C.c_void_p), ("q_token_stride", C.c_int64), ("q_head_stride", C.c_int64),
+        ("k", C.c_void_p), ("k_token_stride", C.c_int64), ("k_head_stride", C.c_int64),
+        ("v", C.c_void_p), ("v_token_stride", C.c_int64), ("v_head_stride", C.c_int64),
+        ("out", C.c_void_p), ("out_token_stride", C.c_int64), ("out_head_stride", C.c_int64),
+        ("cu_q", C.c_void_p), ("cu_k", C.c_void_p), ("scale", C.c_float), ("lse", C.c_void_p),
     ]
 
 
@@ -111,6 +157,19 @@ def lib(path: Path | None = None) -> C.CDLL:
         h.b2g_gemm_splitk_peer.restype = C.c_int
         h.b2g_read_device_error.argtypes = [C.c_int, C.POINTER(C.c_int32)]
         h.b2g_read_device_error.restype = C.c_int
+        h.b2g_block_tables.argtypes = [C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                       C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_int64,
+                                       C.c_int, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p,
+                                       C.c_void_p]
+        h.b2g_block_tables.restype = C.c_int
+        h.b2g_cache_append.argtypes = [C.POINTER(CacheAppendDesc), C.c_void_p]
+        h.b2g_cache_append.restype = C.c_int
+        h.b2g_cache_attention_workspace_bytes.argtypes = [C.POINTER(CacheAttentionDesc)]
+        h.b2g_cache_attention_workspace_bytes.restype = C.c_int64
+        h.b2g_cache_attention.argtypes = [C.POINTER(CacheAttentionDesc), C.c_void_p]
+        h.b2g_cache_attention.restype = C.c_int
+        h.b2g_prompt_attention.argtypes = [C.POINTER(PromptAttentionDesc), C.c_void_p]
+        h.b2g_prompt_attention.restype = C.c_int
         h.b2g_status_string.argtypes = [C.c_int]
         h.b2g_status_string.restype = C.c_char_p
         h.b2g_version.argtypes = []
@@ -238,6 +297,31 @@ def torch_gemm_splitk_peer(A, B, mailboxes, rank, root, epoch):
     from . import native
 
     return native().splitk_peer_matmul(A, B, list(mailboxes), rank, root, epoch)
+
+
+def block_tables(context_lens, new_lens, requests, block_table, table_width, table_ld, free_blocks,
+                 free_capacity, free_count, total_tokens, block_size, slots, cu_seqlens, seq_lens,
+                 free_count_out, stream: int = 0) -> int:
+    return lib().b2g_block_tables(context_lens, new_lens, requests, block_table, table_width,
+                                  table_ld, free_blocks, free_capacity, free_count, total_tokens,
+                                  block_size, slots, cu_seqlens, seq_lens, free_count_out,
+                                  C.c_void_p(stream))
+
+
+def cache_append(desc: CacheAppendDesc, stream: int = 0) -> int:
+    return lib().b2g_cache_append(C.byref(desc), C.c_void_p(stream))
+
+
+def cache_attention_workspace_bytes(desc: CacheAttentionDesc) -> int:
+    return lib().b2g_cache_attention_workspace_bytes(C.byref(desc))
+
+
+def cache_attention(desc: CacheAttentionDesc, stream: int = 0) -> int:
+    return lib().b2g_cache_attention(C.byref(desc), C.c_void_p(stream))
+
+
+def prompt_attention(desc: PromptAttentionDesc, stream: int = 0) -> int:
+    return lib().b2g_prompt_attention(C.byref(desc), C.c_void_p(stream))
 
 
 def read_device_error(device: int = 0) -> int:
