@@ -90,22 +90,29 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
 // As mbar_wait, for waits on a critical path: the thread is suspended in the
 // wait itself (up to the hint, 20 us), so it neither takes issue slots from
 // its neighbours nor stands in a read of the global timer (some 900 cycles)
-// when the phase completes; the timer bounds what 64 such waits do not.
+// when the phase completes; the timer is read at every 64th probe only.  Kept
+// small: it stands at many places of a kernel whose code has to be fetched.
 __device__ __forceinline__ bool mbar_wait_suspended(uint64_t* bar, uint32_t parity,
                                                     volatile int* abort, uint64_t limit_ns) {
+  const uint32_t at = smem_addr(bar);
+  uint64_t t0 = 0;
 #pragma unroll 1
-  for (int i = 0; i < 64; ++i) {
+  for (uint32_t i = 1;; ++i) {
     uint32_t ok;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
         "selp.u32 %0, 1, 0, p;\n\t}"
         : "=r"(ok)
-        : "r"(smem_addr(bar)), "r"(parity), "r"(20000u)
+        : "r"(at), "r"(parity), "r"(20000u)
         : "memory");
     if (ok) return true;
+    if (i % 64 == 0) {
+      const uint64_t t = globaltimer_ns();
+      if (t0 == 0) t0 = t;
+      if (*abort || t - t0 > limit_ns) return false;
+    }
   }
-  return mbar_wait(bar, parity, abort, limit_ns);
 }
 
 // ------------------------------------------------- programmatic dependent launch
