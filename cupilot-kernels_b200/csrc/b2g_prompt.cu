@@ -51,10 +51,7 @@ constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kAskAhead = 2;          // key tiles left to load when the next item is asked for
 constexpr int kItemReaders = kSoftmaxWarps + 3;
 // Of 16 pairs of exponentials, how many run on the FMA units.
-#ifndef POLY
-#define POLY 3
-#endif
-constexpr int kPolyPairs = POLY;
+constexpr int kPolyPairs = 3;
 constexpr float kGrow = 8.f;
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kBoxBytes = 128 * 128;  // 64 columns x 128 rows of 16 bits
@@ -82,6 +79,7 @@ struct Params {
   const int32_t* cu_k;
   int sequences, tokens, tokens_k, heads, kv_heads, group, dim;
   int tile_tokens;                    // tokens of a tile: 128 / group
+  int span;                           // tokens of a work item: two tiles, or one
   int causal;
   int slots;                          // upper bound of tile pairs over all sequences
   float scale_log2;
@@ -255,7 +253,7 @@ __device__ __forceinline__ int keys_of(const Params& p, const Item& it, int tok)
 // Tile pair x of all sequences: sequence s owns the places from
 // cu[s] / span + s on, at least as many as it has pairs; some stay empty.
 __device__ __forceinline__ bool find_item(const Params& p, int x, int head, Item* it) {
-  const int span = 2 * p.tile_tokens;
+  const int span = p.span;
   int lo = 0, hi = p.sequences;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -273,7 +271,7 @@ __device__ __forceinline__ bool find_item(const Params& p, int x, int head, Item
     return t0 < it->qlen ? (keys_of(p, *it, last) + kKeys - 1) / kKeys : 0;
   };
   it->n0 = tiles(it->first);
-  it->n1 = tiles(it->first + p.tile_tokens);
+  it->n1 = span > p.tile_tokens ? tiles(it->first + p.tile_tokens) : 0;
   return it->first >= 0 && it->first < it->qlen;
 }
 
@@ -637,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ni = i ? it.n1 : it.n0;
       const int t0 = it.first + i * p.tile_tokens;
       const int tok = t0 + row_tok;
-      const bool mine = row_tok < p.tile_tokens && tok < it.qlen;
+      const bool mine = row_tok < p.tile_tokens && tok < it.qlen && t0 < it.first + p.span;
       const int limit = keys_of(p, it, tok);
       const int least = keys_of(p, it, t0);      // no row of the tile sees fewer keys
       float m = -INFINITY;                       // in log2 units
@@ -700,6 +698,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float off = m == -INFINITY ? 0.f : -m;
         const uint64_t off2 = pair(off, off);
+        uint64_t odd2 = 0;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t w[16];
@@ -715,10 +714,13 @@ __global__ void __launch_bounds__(kThreads, 1)
               a = exp2_fast(a);
               b = exp2_fast(b);
             }
-            l2 = add2(l2, pair(a, b));
+            // (two chains: one of 64 dependent additions a step was 4 % of the time)
+            uint64_t& sum2 = x & 1 ? odd2 : l2;
+            sum2 = add2(sum2, pair(a, b));
             w[x] = pack<BF16>(a, b);
           }
           tmem_st_x16(ts + c * 16, w);
+          if (c == 3) l2 = add2(l2, odd2);
           if (c & 1) {
             tmem_st_wait();
             ptx::tc_fence_before();
@@ -858,7 +860,10 @@ extern "C" int b2g_prompt_attention(const b2g_prompt_attention_desc* d, b2g_stre
   p.lse = d->lse;
   p.wait_limit_ns = b2g::current_wait_limit_ns();
   p.err = dev.error_word;
-  const int64_t slots = std::max<int64_t>(d->tokens / (2 * p.tile_tokens) + d->sequences, 1);
+  // Two tiles a work item; one where that still leaves no more items than SMs.
+  auto slots_of = [&](int64_t span) { return std::max<int64_t>(d->tokens / span + d->sequences, 1); };
+  p.span = slots_of(p.tile_tokens) * p.kv_heads <= dev.num_sms ? p.tile_tokens : 2 * p.tile_tokens;
+  const int64_t slots = slots_of(p.span);
   if (slots * p.kv_heads > 0x7fffffff) return B2G_ERR_UNSUPPORTED;
   p.slots = static_cast<int>(slots);
   const bool bf = d->dtype == B2G_BF16;
