@@ -544,7 +544,9 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
             vs = __ldg(a.v_scale + static_cast<int64_t>(id) * a.kv_heads + head);
           }
         }
-        if (!ptx::mbar_wait_suspended(&empty[slot], ((n / L::kStages) & 1) ^ 1, abort_flag, a.wait_limit_ns)) {
+        const bool come =
+            ptx::mbar_wait_suspended(&empty[slot], ((n / L::kStages) & 1) ^ 1, abort_flag, a.wait_limit_ns);
+        if (!__all_sync(0xffffffffu, come)) {
           if (lane == 0) fail(a.err, abort_flag, kErrEmpty);
           ok = false;
           break;
@@ -598,7 +600,10 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     load_query<DP, ROWS, E4M3>(s, a, seg.r, head, rg, lane);
     for (int t = seg.t0; t < seg.t1; ++t, ++n) {
       const int slot = n % L::kStages;
-      if (!ptx::mbar_wait_suspended(&full[slot], (n / L::kStages) & 1, abort_flag, a.wait_limit_ns)) {
+      // (one answer for the warp: it stays converged; after a failure the waits to come fail at once)
+      const bool come =
+          ptx::mbar_wait_suspended(&full[slot], (n / L::kStages) & 1, abort_flag, a.wait_limit_ns);
+      if (!__all_sync(0xffffffffu, come)) {
         if (lane == 0) fail(a.err, abort_flag, kErrFull);
         break;
       }

@@ -354,10 +354,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   ptx::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
+  // A wait of a whole warp: one answer, so that it stays converged where a wait gives up.
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity, volatile int* abort) {
+    const bool come = ptx::mbar_wait_suspended(bar, parity, abort, p.wait_limit_ns);
+    return __all_sync(0xffffffffu, come) != 0;
+  };
   // The k-th item of this CTA, for the warps that work on it.
   auto get_item = [&](uint32_t k, Item* it) {
-    const bool come = ptx::mbar_wait_suspended(&item_full[k & 1], (k >> 1) & 1, abort_flag, p.wait_limit_ns);
-    if (!__all_sync(0xffffffffu, come)) {
+    if (!warp_wait(&item_full[k & 1], (k >> 1) & 1, abort_flag)) {
       if (lane == 0) fail(p.err, abort_flag, kErrItem);
       return false;
     }
@@ -380,7 +384,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // Late tiles see the most keys: they go first.
         if (p.sequences > 0 && find_item(p, p.slots - 1 - w / p.kv_heads, w % p.kv_heads, &it)) {
           it.more = 1;
-          if (!ptx::mbar_wait_suspended(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+          if (!warp_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag)) {
             if (lane == 0) fail(p.err, abort_flag, kErrItem);
             break;
           }
@@ -390,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           // Another CTA's work is taken over when this item's last key tiles are on their way: early
           // enough to hide the question, late enough that whoever is done first takes what is left.
-          if (!ptx::mbar_wait_suspended(next_wanted, k & 1, abort_flag, p.wait_limit_ns)) {
+          if (!warp_wait(next_wanted, k & 1, abort_flag)) {
             if (lane == 0) fail(p.err, abort_flag, kErrNext);
             break;
           }
@@ -402,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ptx::clc_try_cancel(next_answer, next_full);
         }
         volatile int never = 0;                  // (the answer lands before the CTA leaves)
-        if (!ptx::mbar_wait_suspended(next_full, asked & 1, &never, p.wait_limit_ns)) {
+        if (!warp_wait(next_full, asked & 1, &never)) {
           if (lane == 0) fail(p.err, abort_flag, kErrNext);
           break;
         }
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         more = ptx::clc_answer(next_answer, &w);
         __syncwarp();
       }
-      if (ptx::mbar_wait_suspended(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag, p.wait_limit_ns)) {
+      if (warp_wait(&item_empty[k & 1], ((k >> 1) & 1) ^ 1, abort_flag)) {
         if (lane == 0) {
           item_at(k)->more = 0;
           ptx::mbar_arrive(&item_full[k & 1]);
@@ -489,8 +493,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int n = max(it.n0, it.n1);
         if (n * kKeys > it.klen) {
           const uint32_t e = used + 2 * (n - 1) + 1;
-          const bool come = ptx::mbar_wait_suspended(tail_there, tails++ & 1, abort_flag, p.wait_limit_ns);
-          if (!__all_sync(0xffffffffu, come)) {
+          if (!warp_wait(tail_there, tails++ & 1, abort_flag)) {
             if (lane == 0) fail(p.err, abort_flag, kErrFull);
             ok = false;
             break;
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY;                       // in log2 units
       uint64_t l2 = 0;                           // the sum, in two parts
       for (int j = 0; j < ni; ++j, ++steps) {
-        if (!ptx::mbar_wait_suspended(&s_full[i], steps & 1, abort_flag, p.wait_limit_ns)) {
+        if (!warp_wait(&s_full[i], steps & 1, abort_flag)) {
           if (lane == 0) fail(p.err, abort_flag, kErrS);
           ok = false;
           break;
@@ -678,7 +681,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           unpair(l2, la, lb);
           l2 = pair(la * corr, lb * corr);
           if (j > 0) {
-            if (!ptx::mbar_wait_suspended(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+            if (!warp_wait(&o_done[i], (steps - 1) & 1, abort_flag)) {
               if (lane == 0) fail(p.err, abort_flag, kErrO);
               ok = false;
               break;
@@ -733,7 +736,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int h = it.head * p.group + g;
       uint16_t* out = p.out + t * p.out_token + h * p.out_head;
       if (ok && ni > 0) {
-        if (!ptx::mbar_wait_suspended(&o_done[i], (steps - 1) & 1, abort_flag, p.wait_limit_ns)) {
+        if (!warp_wait(&o_done[i], (steps - 1) & 1, abort_flag)) {
           if (lane == 0) fail(p.err, abort_flag, kErrO);
           ok = false;
         }
