@@ -557,6 +557,122 @@ def test_prompt_on_another_stream(ops):
     assert torch.equal(got, want)
 
 
+# ------------------------------------------- long caches, streams and graphs
+@pytest.mark.parametrize("codes", CODES, ids=_ids)
+def test_cache_past_32_bits(ops, codes):
+    """Blocks more than 2^32 codes from the cache's start: written, and read again."""
+    h, d, bs, n = 8, 128, 16, 280000                 # 4.6 G codes each of K and V
+    kc, vc = (torch.empty(n, h, bs, d, dtype=torch.uint8, device="cuda").view(codes) for _ in range(2))
+    ks, vs = (torch.zeros(n, h, device="cuda") for _ in range(2))
+    g = torch.Generator().manual_seed(20)
+    ids = [n - 1, 3, n - 7, 150000]
+    k, v = (torch.randn(60, h, d, generator=g).half() for _ in range(2))
+    slots = [ids[t // bs] * bs + t % bs for t in range(60)]
+    ops.cache_append(k.cuda(), v.cuda(), _dev(slots, torch.int64), kc, vc, ks, vs)
+    kv = []
+    for x, c, s in ((k, kc, ks), (v, vc, vs)):
+        want, scale = torch.zeros(4, h, bs, d, dtype=torch.uint8).view(codes), torch.zeros(4, h)
+        _append_oracle(x, list(range(60)), want, scale)
+        at = torch.tensor(ids, device="cuda")
+        assert torch.equal(s[at].cpu(), scale)
+        got = c.view(torch.uint8)[at].cpu().transpose(1, 2).reshape(64, h, d)[:60]
+        assert torch.equal(got, want.view(torch.uint8).transpose(1, 2).reshape(64, h, d)[:60])
+        kv.append((want.double() * scale.double()[:, :, None, None]).transpose(1, 2).reshape(64, h, d)[:60])
+    q = torch.randn(1, 2 * h, d, generator=g).half()
+    out = ops.cache_attention(q.cuda(), kc, vc, ks, vs, _dev([ids]), _dev([60]))
+    _close(out, _attend(q.double(), *kv, d ** -0.5)[0], torch.float16)
+    _no_error(ops)
+
+
+def test_prompt_past_32_bits(ops):
+    """Rows 2^24 elements apart: the last ones begin 3.3 G elements behind the first."""
+    n, h, d, pitch = 200, 2, 64, 1 << 24
+    buf = torch.empty(n * pitch, dtype=torch.float16, device="cuda")
+    q, k, v = (torch.as_strided(buf, (n, h, d), (pitch, d, 1), i * 4096) for i in range(3))
+    g = torch.Generator().manual_seed(21)
+    for x in (q, k, v):
+        x.copy_(torch.randn(n, h, d, generator=g))
+    cu = _dev([0, 77, n])
+    got = ops.prompt_attention(q, k, v, cu)
+    assert torch.equal(got, ops.prompt_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu))
+    _no_error(ops)
+
+
+def _step_state(seed):
+    g = torch.Generator().manual_seed(seed)
+    lens = [40, 0, 17, 100]
+    held = [-(-n // 16) for n in lens]
+    order = torch.randperm(sum(held) + 6, generator=g).int()
+    table = torch.full((4, 10), -1, dtype=torch.int32)
+    at = 0
+    for r, n in enumerate(held):
+        table[r, :n] = order[at:at + n]
+        at += n
+    caches = []
+    for _ in range(2):
+        caches += _random_cache(g, len(order), 2, 16, 64, torch.int8)
+    q, k, v = (torch.randn(4, n, 64, generator=g).half() for n in (4, 2, 2))
+    kc, ks, vc, vs = (x.cuda() for x in caches)
+    return dict(lens=_dev(lens), one=_dev([1] * 4), table=table.cuda(), free=order[at:].clone().cuda(),
+                count=_dev([len(order) - at]), kc=kc, ks=ks, vc=vc, vs=vs, q=q.cuda(), k=k.cuda(), v=v.cuda())
+
+
+def _step(ops, s):
+    slots, cu, lens, left = ops.block_tables(s["lens"], s["one"], s["table"], s["free"], s["count"], 4, 16)
+    ops.cache_append(s["k"], s["v"], slots, s["kc"], s["vc"], s["ks"], s["vs"])
+    out = ops.cache_attention(s["q"], s["kc"], s["vc"], s["ks"], s["vs"], s["table"], lens)
+    own = ops.prompt_attention(s["q"], s["k"], s["v"], cu)
+    return slots, lens, left, out, own, s["kc"], s["ks"], s["table"]
+
+
+def test_step_on_another_stream(ops):
+    want = _step(ops, _step_state(30))
+    state = _step_state(30)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        got = _step(ops, state)
+    stream.synchronize()
+    for a, b in zip(want, got):
+        assert torch.equal(a, b)
+
+
+def test_step_in_a_graph(ops):
+    want = _step(ops, _step_state(31))
+    warm, state = _step_state(32), _step_state(31)
+    _step(ops, warm)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _step(ops, state)
+    fresh = _step_state(31)                          # the capture ran nothing
+    for name, x in state.items():
+        assert torch.equal(x, fresh[name])
+    for _ in range(2):                               # a step over the same lengths repeats itself
+        graph.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            assert torch.equal(a, b)
+    _no_error(ops)
+
+
+def test_prompt_then_one_token_agree(ops):
+    """The last row of a prompt's attention is what one token sees over the cache of the others, but
+    for the cache's 8 bits (int8: about 1 % of a value's standard deviation, in K and in V)."""
+    g = torch.Generator().manual_seed(33)
+    n, h, d = 300, 2, 128
+    q, k, v = (torch.randn(n, x, d, generator=g).half().cuda() for x in (4 * h, h, h))
+    blocks = -(-n // 16)
+    kc, vc = (torch.zeros(blocks, h, 16, d, dtype=torch.int8, device="cuda") for _ in range(2))
+    ks, vs = (torch.zeros(blocks, h, device="cuda") for _ in range(2))
+    ops.cache_append(k, v, torch.arange(n, device="cuda"), kc, vc, ks, vs)
+    table = torch.arange(blocks, dtype=torch.int32, device="cuda")[None]
+    token, lse = ops.cache_attention(q[-1:], kc, vc, ks, vs, table, _dev([n]), return_lse=True)
+    prompt, plse = ops.prompt_attention(q, k, v, _dev([0, n]), return_lse=True)
+    assert ((token - prompt[-1:]).norm() / prompt[-1:].norm()) <= 0.04
+    assert (lse - plse[-1:]).abs().max() <= 0.04
+
+
 # ----------------------------------------------------------------- refusals
 def test_refusals(ops):
     q = torch.randn(4, 4, 64, device="cuda").half()
