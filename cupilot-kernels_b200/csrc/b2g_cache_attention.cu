@@ -322,24 +322,35 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
     }
 }
 
-template <int DP, int ROWS, bool E4M3>
-__device__ __forceinline__ void load_query(State<DP, ROWS>& s, const Args& a, int r, int head,
-                                           int rg, int lane) {
-  constexpr int N = ROWS / 8;
+// A segment's queries as they stand in memory: head 8 n + g, dims DP/4 c ...
+template <int DP, int ROWS>
+__device__ __forceinline__ void fetch_query(uint4 (&raw)[ROWS / 8][DP / 32], const Args& a, int r, int head,
+                                            int rg, int lane) {
   const int g = lane >> 2, c = lane & 3;
 #pragma unroll
+  for (int n = 0; n < ROWS / 8; ++n) {
+    const int row = rg * ROWS + 8 * n + g, d0 = DP / 4 * c;
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) + r * a.q_row +
+                        static_cast<int64_t>(head * a.group + row) * a.q_head + d0;
+#pragma unroll
+    for (int j = 0; j < DP / 32; ++j)
+      raw[n][j] = row < a.group && d0 + 8 * j < a.dim ? __ldg(reinterpret_cast<const uint4*>(q + 8 * j))
+                                                      : make_uint4(0, 0, 0, 0);
+  }
+}
+
+template <int DP, int ROWS, bool E4M3>
+__device__ __forceinline__ void take_query(State<DP, ROWS>& s, const uint4 (&raw)[ROWS / 8][DP / 32],
+                                           const Args& a, int lane) {
+  constexpr int N = ROWS / 8;
+  const int c = lane & 3;
+#pragma unroll
   for (int n = 0; n < N; ++n) {
-    const int row = rg * ROWS + 8 * n + g;
     float x[DP / 4];
     float most = 0.f;
-    const int d0 = DP / 4 * c;           // this lane's dims
 #pragma unroll
     for (int j = 0; j < DP / 32; ++j) {
-      uint4 w = make_uint4(0, 0, 0, 0);
-      if (row < a.group && d0 + 8 * j < a.dim)
-        w = __ldg(reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(a.q) + r * a.q_row +
-                                                 static_cast<int64_t>(head * a.group + row) * a.q_head +
-                                                 d0 + 8 * j));
+      const uint4 w = raw[n][j];
       const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -585,8 +596,19 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
   const int g = lane >> 2, c = lane & 3;
   uint32_t n = 0;
   bool first = true;
-  while (seg.next(a)) {
+  // With rows of 64 bytes the next segment's queries are fetched before this one is joined (48
+  // ragged requests: 44.3 -> 42.2 us); with 128 the registers for it are not there (60.5 -> 64.0).
+  constexpr bool kAhead = DP == 64;
+  uint4 raw[N][DP / 32];
+  auto fetch = [&]() {
+    fetch_query<DP, ROWS>(raw, a, seg.r, seg.head / a.row_groups, seg.head % a.row_groups, lane);
+  };
+  bool more = seg.next(a);
+  if (more && kAhead) fetch();
+  while (more) {
     const int head = seg.head / a.row_groups, rg = seg.head % a.row_groups;
+    const int r = seg.r, len = seg.len, t0 = seg.t0, t1 = seg.t1;
+    const bool whole = t0 == 0 && t1 == seg.tiles;
     State<DP, ROWS> s;
 #pragma unroll
     for (int i = 0; i < N; ++i)
@@ -597,8 +619,9 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
     for (int i = 0; i < N; ++i)
 #pragma unroll
       for (int t = 0; t < DP / 16; ++t) s.o[i][t][0] = s.o[i][t][1] = s.o[i][t][2] = s.o[i][t][3] = 0.f;
-    load_query<DP, ROWS, E4M3>(s, a, seg.r, head, rg, lane);
-    for (int t = seg.t0; t < seg.t1; ++t, ++n) {
+    if (!kAhead) fetch();
+    take_query<DP, ROWS, E4M3>(s, raw, a, lane);
+    for (int t = t0; t < t1; ++t, ++n) {
       const int slot = n % L::kStages;
       // (one answer for the warp: it stays converged; after a failure the waits to come fail at once)
       const bool come =
@@ -608,7 +631,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
         break;
       }
       constexpr int P = pieces(DP);
-      const int left = seg.len - t * L::kTile - warp * 16 * P;
+      const int left = len - t * L::kTile - warp * 16 * P;
       float2 sc[P];
 #pragma unroll
       for (int x = 0; x < P; ++x) sc[x] = scales[slot * L::kPieces + warp * P + x];
@@ -619,6 +642,9 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
       __syncwarp();
       if (lane == 0) ptx::mbar_arrive(&empty[slot]);
     }
+
+    more = seg.next(a);
+    if (more && kAhead) fetch();
 
     // Join the four warps.
 #pragma unroll
@@ -640,7 +666,6 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
                           s.o[i][t + 1][2 + h] * s.unit);
       }
     asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
-    const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
     const int rows = min(ROWS, a.group - rg * ROWS);
     for (int i = tid; i < rows * DP; i += kWarps * 32) {
@@ -658,7 +683,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
       }
       if (whole) {
         const int64_t j =
-            static_cast<int64_t>(seg.r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
+            static_cast<int64_t>(r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
         if (d < a.dim) store_out(a, j * a.dim + d, l > 0.f ? o / l : (l == 0.f ? 0.f : l));
         if (d == 0 && a.lse) a.lse[j] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       } else {
@@ -674,82 +699,95 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
   }
 }
 
-// Joins the parts of what the cuts divided, one CTA for each query head; a
-// warp takes every warps-th part, a lane DP / 32 dims.  Requests without
-// tokens get their zeros here.
-template <int DP, int ROWS>
+// Joins the parts of what the cuts divided, and writes the zeros of requests
+// without tokens.  SPREAD (few heads, so many parts each): a CTA for each
+// query head, its warps take every warps-th part.  Else a CTA for each
+// request and virtual head, and a warp for each of its rows.
+template <int DP, int ROWS, bool SPREAD>
 __global__ void cache_join_kernel(const Args a) {
-  extern __shared__ float sm[];          // [warps][DP + 1]
+  extern __shared__ float sm[];          // SPREAD: [warps][DP + 1]
   ptx::griddep_wait();
   const int heads = a.kv_heads * a.row_groups;
-  const int j = blockIdx.x % (a.kv_heads * a.group), r = blockIdx.x / (a.kv_heads * a.group);
-  const int head = j / a.group, row = j % a.group, rg = row / ROWS, y = row % ROWS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int all = SPREAD ? a.kv_heads * a.group : heads;
+  const int r = blockIdx.x / all, j = blockIdx.x % all;
+  const int head = SPREAD ? j / a.group : j / a.row_groups;
+  const int rg = SPREAD ? j % a.group / ROWS : j % a.row_groups;
   const int before = a.prefix[r], tiles = a.prefix[r + 1] - before;
-  const int64_t at = static_cast<int64_t>(blockIdx.x);
-  if (tiles == 0) {
-    for (int d = threadIdx.x; d < a.dim; d += blockDim.x) store_out(a, at * a.dim + d, 0.f);
-    if (threadIdx.x == 0 && a.lse) a.lse[at] = -INFINITY;
-    return;
-  }
   const int64_t units = static_cast<int64_t>(a.prefix[a.requests]) * heads;
   const int64_t share = (units + a.grid - 1) / a.grid;
   const int64_t u0 = static_cast<int64_t>(before) * heads +
                      static_cast<int64_t>(head * a.row_groups + rg) * tiles;
-  const int c0 = static_cast<int>(u0 / share), c1 = static_cast<int>((u0 + tiles - 1) / share);
-  if (c0 == c1) return;
-  // The first part is its CTA's first segment only where it begins there.
-  auto slot_of = [&](int c) {
-    return (2ll * c + (c == c0 && u0 != c0 * share ? 1 : 0)) * ROWS + y;
-  };
-  float m = -INFINITY;
-  for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_m[slot_of(c)]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-  // A warp's parts: their weights side by side in the lanes, their rows kJoin at a time.
-  float l = 0.f, acc[DP / 32];
-#pragma unroll
-  for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
-  for (int base = c0 + warp; base <= c1; base += 32 * warps) {
-    const int own = base + lane * warps;
-    float e = 0.f;
-    if (own <= c1) {
-      const float pm = a.part_m[slot_of(own)];
-      e = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
-      l += e * a.part_l[slot_of(own)];
-    }
-    const int n = min(32, (c1 - base) / warps + 1);
-    for (int k = 0; k < n; k += kJoin) {
-      float v[kJoin][DP / 32];
-#pragma unroll
-      for (int x = 0; x < kJoin; ++x) {
-        const int64_t slot = slot_of(base + (k + x) * warps);
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i)
-          v[x][i] = k + x < n ? a.part_o[slot * DP + lane + 32 * i] : 0.f;
-      }
-#pragma unroll
-      for (int x = 0; x < kJoin; ++x) {
-        const float w = __shfl_sync(0xffffffffu, e, (k + x) & 31);
-#pragma unroll
-        for (int i = 0; i < DP / 32; ++i) acc[i] += (k + x < n ? w : 0.f) * v[x][i];
-      }
-    }
+  int c0 = 0, c1 = 0;
+  bool late = false;                     // the first part is not its CTA's first segment
+  if (tiles > 0) {
+    c0 = static_cast<int>(u0 / share), c1 = static_cast<int>((u0 + tiles - 1) / share);
+    late = u0 != c0 * share;
+    if (c0 == c1) return;                // one CTA did it all
   }
+  const int first = SPREAD ? warp : 0, step = SPREAD ? warps : 1;
+  const int last_row = SPREAD ? j % a.group % ROWS + 1 : min(ROWS, a.group - rg * ROWS);
+  for (int y = SPREAD ? last_row - 1 : warp; y < last_row; y += SPREAD ? ROWS : warps) {
+    const int64_t at = static_cast<int64_t>(r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
+    auto slot_of = [&](int c) { return (2ll * c + (c == c0 && late ? 1 : 0)) * ROWS + y; };
+    float m = -INFINITY, l = 0.f, acc[DP / 32];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+    for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
+    if (tiles > 0) {
+      for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_m[slot_of(c)]);
 #pragma unroll
-  for (int i = 0; i < DP / 32; ++i) sm[warp * (DP + 1) + lane + 32 * i] = acc[i];
-  if (lane == 0) sm[warp * (DP + 1) + DP] = l;
-  __syncthreads();
-  for (int d = threadIdx.x; d < a.dim; d += blockDim.x) {
-    float lt = 0.f, ot = 0.f;
-    for (int w = 0; w < warps; ++w) {
-      lt += sm[w * (DP + 1) + DP];
-      ot += sm[w * (DP + 1) + d];
+      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      // A warp's parts: their weights side by side in the lanes, their rows kJoin at a time.
+      for (int base = c0 + first; base <= c1; base += 32 * step) {
+        const int own = base + lane * step;
+        float e = 0.f;
+        if (own <= c1) {
+          const float pm = a.part_m[slot_of(own)];
+          e = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
+          l += e * a.part_l[slot_of(own)];
+        }
+        const int n = min(32, (c1 - base) / step + 1);
+        for (int k = 0; k < n; k += kJoin) {
+          float v[kJoin][DP / 32];
+#pragma unroll
+          for (int x = 0; x < kJoin; ++x) {
+            const int64_t slot = slot_of(base + (k + x) * step);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i)
+              v[x][i] = k + x < n ? a.part_o[slot * DP + lane + 32 * i] : 0.f;
+          }
+#pragma unroll
+          for (int x = 0; x < kJoin; ++x) {
+            const float w = __shfl_sync(0xffffffffu, e, (k + x) & 31);
+#pragma unroll
+            for (int i = 0; i < DP / 32; ++i) acc[i] += (k + x < n ? w : 0.f) * v[x][i];
+          }
+        }
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
     }
-    store_out(a, at * a.dim + d, lt > 0.f ? ot / lt : (lt == 0.f ? 0.f : lt));
-    if (d == 0 && a.lse) a.lse[at] = lt == 0.f ? -INFINITY : (m + log2f(lt)) * 0.6931471805599453f;
+    if (SPREAD) {
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) sm[warp * (DP + 1) + lane + 32 * i] = acc[i];
+      if (lane == 0) sm[warp * (DP + 1) + DP] = l;
+      __syncthreads();
+      if (warp > 0) return;
+      l = 0.f;
+#pragma unroll
+      for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
+      for (int w = 0; w < warps; ++w) {
+        l += sm[w * (DP + 1) + DP];
+#pragma unroll
+        for (int i = 0; i < DP / 32; ++i) acc[i] += sm[w * (DP + 1) + lane + 32 * i];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < DP / 32; ++i) {
+      const int d = lane + 32 * i;
+      if (d < a.dim) store_out(a, at * a.dim + d, l > 0.f ? acc[i] / l : (l == 0.f ? 0.f : l));
+    }
+    if (lane == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
 }
 
@@ -829,14 +867,16 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
   cfg.numAttrs = 0;
   if (cudaLaunchKernelEx(&cfg, cache_attention_kernel<DP, ROWS, E4M3>, mk, mv, a) != cudaSuccess)
     return B2G_ERR_LAUNCH;
-  const int64_t heads = static_cast<int64_t>(a.kv_heads) * a.group;
-  // Parts of a head, were all lengths alike.
-  const int warps = a.grid > 16 * a.requests * a.kv_heads * a.row_groups ? 16 : 4;
+  // Parts of a head, were all lengths alike: from 8 on they are spread over 16 warps.
+  const int64_t heads = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups;
+  const bool spread = a.grid > 8 * heads;
+  const int warps = spread ? 16 : std::min(4, ROWS);
   cfg.numAttrs = b2g::pdl_enabled() ? 1 : 0;
-  cfg.gridDim = dim3(static_cast<unsigned>(a.requests * heads), 1, 1);
+  cfg.gridDim = dim3(static_cast<unsigned>(spread ? static_cast<int64_t>(a.requests) * a.kv_heads * a.group : heads), 1, 1);
   cfg.blockDim = dim3(warps * 32, 1, 1);
-  cfg.dynamicSmemBytes = warps * (DP + 1) * sizeof(float);
-  if (cudaLaunchKernelEx(&cfg, cache_join_kernel<DP, ROWS>, a) != cudaSuccess) return B2G_ERR_LAUNCH;
+  cfg.dynamicSmemBytes = spread ? warps * (DP + 1) * sizeof(float) : 0;
+  auto* join = spread ? cache_join_kernel<DP, ROWS, true> : cache_join_kernel<DP, ROWS, false>;
+  if (cudaLaunchKernelEx(&cfg, join, a) != cudaSuccess) return B2G_ERR_LAUNCH;
   return cudaGetLastError() == cudaSuccess ? B2G_OK : B2G_ERR_LAUNCH;
 }
 
