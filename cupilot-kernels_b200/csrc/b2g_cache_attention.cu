@@ -38,12 +38,16 @@ namespace ptx = b2g::ptx;
 
 inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-constexpr int kWarps = 4;                       // consumers
-constexpr int kThreads = (kWarps + 1) * 32;     // and the producer
+// Consumer warps of a CTA; the producer is one more.  Two CTAs of six warps
+// fill an SM's registers where 16 heads' sums of 128 dims take 168 a thread.
+__host__ __device__ constexpr int consumers(int dp, int rows) { return dp == 128 && rows == 16 ? 5 : 4; }
 // Pieces of 16 tokens that a consumer warp takes from a stage: with rows of 64
 // bytes two at once, so that their chains of dependent products overlap.
 __host__ __device__ constexpr int pieces(int dp) { return dp == 64 ? 2 : 1; }
-__host__ __device__ constexpr int tile_tokens(int dp) { return 16 * kWarps * pieces(dp); }   // tokens of a stage
+// Tokens of a stage.
+__host__ __device__ constexpr int tile_tokens(int dp, int rows) {
+  return 16 * consumers(dp, rows) * pieces(dp);
+}
 constexpr float kGrow = 8.f;           // a maximum may be passed by 2^8 before the sums are rescaled
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kJoin = 4;                     // rows of parts that a joining warp loads at once
@@ -55,17 +59,21 @@ enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
 template <int DP, int ROWS>
 struct Smem {
   static constexpr int kStages = 3;
-  static constexpr int kTile = tile_tokens(DP);
+  static constexpr int kWarps = consumers(DP, ROWS), kThreads = (kWarps + 1) * 32;
+  static constexpr int kTile = tile_tokens(DP, ROWS);
   static constexpr int kPieces = kTile / 16;
   static constexpr int kSideBytes = kTile * DP;             // K or V of a stage
   static constexpr int kStageBytes = 2 * kSideBytes;
   static constexpr int kOffScales = kStages * kStageBytes;  // [stage][piece]{k scale, v scale}
   static constexpr int kOffBars = kOffScales + kStages * kPieces * 8;
   static constexpr int kOffMisc = kOffBars + 2 * kStages * 8;
-  static constexpr int kOffJoin = kOffMisc + 64;            // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
+  static constexpr int kOffJoin = (kOffMisc + 64 + 15) / 16 * 16;   // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
   static constexpr int kOffO = kOffJoin + 2 * kWarps * ROWS * 4;
   static constexpr int kBytes = kOffO + kWarps * ROWS * DP * 4 + 1024;
   static constexpr int kCtas = ROWS == 8 ? 3 : 2;           // a multiprocessor
+  static_assert(kSideBytes % 1024 == 0 && kOffScales % 8 == 0 && kOffBars % 8 == 0 && kOffO % 16 == 0,
+                "swizzle atoms, float2 scales, barriers, float4 sums");
+  static_assert(kCtas * (kBytes + 1024) <= 227 * 1024 + 1024, "shared memory of an SM");
 };
 
 struct Args {
@@ -400,9 +408,9 @@ __device__ __forceinline__ void store_out(const Args& a, int64_t at, float v) {
 // Tiles before each request: every thread sums a run of requests, the runs'
 // sums are scanned.  Returns the total; *run is the sum before this thread's
 // run, *lo and *hi the run.
-template <int TILE>
+template <int TILE, int THREADS>
 __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo, int* hi, int* run) {
-  const int per = (a.requests + kThreads - 1) / kThreads;
+  const int per = (a.requests + THREADS - 1) / THREADS;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   *lo = min(a.requests, static_cast<int>(threadIdx.x) * per);
   *hi = min(a.requests, *lo + per);
@@ -418,7 +426,7 @@ __device__ __forceinline__ int scan_tiles(const Args& a, int* warp_sum, int* lo,
   __syncthreads();
   int before = 0, total = 0;
 #pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
+  for (int w = 0; w < THREADS / 32; ++w) {
     if (w < warp) before += warp_sum[w];
     total += warp_sum[w];
   }
@@ -458,11 +466,11 @@ __device__ __forceinline__ void fail(int* err, volatile int* abort, int code) {
 }
 
 template <int DP, int ROWS, bool E4M3>
-__global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
+__global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCtas)
     cache_attention_kernel(const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const Args a) {
   using L = Smem<DP, ROWS>;
-  constexpr int N = ROWS / 8;
+  constexpr int N = ROWS / 8, kWarps = L::kWarps;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -488,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, Smem<DP, ROWS>::kCtas)
   }
 
   int lo, hi, run;
-  const int total = scan_tiles<L::kTile>(a, warp_sum, &lo, &hi, &run);
+  const int total = scan_tiles<L::kTile, L::kThreads>(a, warp_sum, &lo, &hi, &run);
   Segments<L::kTile> seg;
   seg.heads = a.kv_heads * a.row_groups;
   const int64_t units = static_cast<int64_t>(total) * seg.heads;
@@ -800,7 +808,7 @@ int check(const b2g_cache_attention_desc* d) {
   if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return B2G_ERR_INVALID_ARG;
   if (d->block_size < 16 || d->block_size > 256 || (d->block_size & (d->block_size - 1)) ||
       d->dim % 16 || d->dim > 128 || d->num_blocks > 0x7fffffff ||
-      d->table_width * d->block_size > 0x7fffffc0 || d->requests > (1 << 20) ||
+      d->table_width * d->block_size > 0x7fffff00 || d->requests > (1 << 20) ||
       d->num_blocks * d->kv_heads * d->block_size > 0x7fffffff || d->heads > (1 << 16) || d->requests * d->heads > 0x7fffffff)
     return B2G_ERR_UNSUPPORTED;
   return B2G_OK;
@@ -818,7 +826,7 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   w.dp = d->dim <= 64 ? 64 : 128;
   w.row_groups = static_cast<int>(cdiv(group, w.rows));
   const int64_t most = d->requests * d->kv_heads * w.row_groups *
-                       std::max<int64_t>(cdiv(d->table_width * d->block_size, tile_tokens(w.dp)), 1);
+                       std::max<int64_t>(cdiv(d->table_width * d->block_size, tile_tokens(w.dp, w.rows)), 1);
   w.grid = static_cast<int>(std::min<int64_t>(
       std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * (w.rows == 8 ? Smem<128, 8>::kCtas : Smem<128, 16>::kCtas)));
   auto pad = [](int64_t n) { return cdiv(n, 256) * 256; };
@@ -860,17 +868,17 @@ int launch(const CUtensorMap& mk, const CUtensorMap& mv, const Args& a, cudaStre
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.grid), 1, 1);
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(L::kThreads, 1, 1);
   cfg.dynamicSmemBytes = L::kBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 0;
   if (cudaLaunchKernelEx(&cfg, cache_attention_kernel<DP, ROWS, E4M3>, mk, mv, a) != cudaSuccess)
     return B2G_ERR_LAUNCH;
-  // Parts of a head, were all lengths alike: from 8 on they are spread over 16 warps.
+  // Parts of a head, were all lengths alike: from 8 on they are spread over 4 warps, from 32 over 16.
   const int64_t heads = static_cast<int64_t>(a.requests) * a.kv_heads * a.row_groups;
   const bool spread = a.grid > 8 * heads;
-  const int warps = spread ? 16 : std::min(4, ROWS);
+  const int warps = a.grid > 32 * heads ? 16 : 4;
   cfg.numAttrs = b2g::pdl_enabled() ? 1 : 0;
   cfg.gridDim = dim3(static_cast<unsigned>(spread ? static_cast<int64_t>(a.requests) * a.kv_heads * a.group : heads), 1, 1);
   cfg.blockDim = dim3(warps * 32, 1, 1);
@@ -937,7 +945,10 @@ extern "C" int b2g_cache_attention(const b2g_cache_attention_desc* d, b2g_stream
   a.grid = w.grid;
   a.wait_limit_ns = b2g::current_wait_limit_ns();
   a.err = dev.error_word;
-  a.box_rows = static_cast<int>(std::min<int64_t>(d->block_size, tile_tokens(w.dp)));
+  // (a stage of 80 tokens is a whole number of 16 rows only)
+  a.box_rows = consumers(w.dp, w.rows) == 4
+                   ? static_cast<int>(std::min<int64_t>(d->block_size, tile_tokens(w.dp, w.rows)))
+                   : 16;
   CUtensorMap mk = {}, mv = {};
   const int64_t cache_rows = d->num_blocks * d->kv_heads * d->block_size;
   if (d->num_blocks > 0 && (!make_map(&mk, d->k_cache, d->dim, cache_rows, w.dp, a.box_rows) ||
