@@ -20,6 +20,19 @@
 // tiles are laid end to end and cut into equal ranges, one a CTA, so ragged
 // lengths fill the GPU evenly; what a cut divides is joined by a second small
 // kernel.
+//
+// Measured (GB/s of codes, 6547 being the card's copy rate):
+//   64 requests of 14000 to 31000 tokens, 8 kv heads, 32 heads, dim 128, int8:
+//   465 us, 6510 GB/s; 0.53 ms once the power limit lowers the clock
+//   1 request of 150001 tokens, 4 kv heads, 32 heads, e4m3: 38 us, 4070 GB/s
+//   (some 10 us are start, the cuts' partial results and their join)
+//   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 42 us,
+//   3170 GB/s (the consumers' chains of dependent products, not the loads)
+//   1 request of 997 tokens: 9.5 us, two launches and a handful of dependent
+//   loads
+// K as the first operand instead of q halves the products (8 heads of 16 rows
+// were empty): 822 -> 475 us together with the TMA ring, whose place registers
+// had before.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

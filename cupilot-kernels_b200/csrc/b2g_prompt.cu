@@ -22,9 +22,22 @@
 // The maximum is taken over only where it grew by more than 2^8 (P stays
 // within 16 bits' range, l and O are fp32): then, rarely, the softmax warps
 // rescale O themselves.
-// Bound by the exponentials beside the products: a pair of tiles has 2^15 of
-// them against 2048 cycles of tensor core work (dim 128), and the special
-// function unit gives 16 a cycle; part of them is computed on the FMA units.
+// What bounds it: a pair of tiles has 2^15 exponentials against 2048 cycles of
+// tensor core work (dim 128); the special function unit gives 16 a cycle, so
+// 3 of 16 are computed on the FMA units (0: 1 to 2 % slower, 5: 5 %).  Beside
+// that a tile's chain softmax - P V - Q K^T, some 1500 + 1024 cycles and four
+// barriers, sets the pace of a step (2700 to 3000 cycles; a third tile has no
+// room in tensor memory).  Measured:
+//   16384 tokens, 16 heads on 4, dim 128, bf16: 0.83 ms, 1320 TFLOP/s, in a
+//   short burst (the card's cuBLAS burst is 1658); 0.96 ms, 1150, once the
+//   power limit holds the clock at 1.6 GHz (cuBLAS then: 1384)
+//   6 prompts of 700 to 2300 tokens, 32 heads on 8: 0.12 ms, 910 TFLOP/s
+// Tried and slower: two threads to a row (four softmax warps a scheduler: S
+// read twice or registers spilled, +15 %), a thread for each tile's products
+// (both tiles' softmax then fall on the same cycles, +25 %), branches around
+// key columns past the diagonal (+4 %, the compiler no longer interleaves the
+// columns), O staged through shared memory for whole-line stores (-3 % where
+// items are short, +2 % where they are long).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

@@ -91,7 +91,8 @@ B2G_API int b2g_cache_append(const b2g_cache_append_desc* desc, b2g_stream_t str
  *   out[r][j] = sum_n softmax_n(scale * q[r][j] . K[r][n]) V[r][n],
  *   n < seq_lens[r], token n in block block_table[r][n / block_size]
  * Lengths are cut to table_width * block_size; a block number outside the
- * cache leaves its tokens out.  A request without tokens gives zeros, and
+ * cache leaves its tokens out.  num_blocks * kv_heads * block_size, the rows
+ * that the kernel counts, stays below 2^31 (so does table_width * block_size).  A request without tokens gives zeros, and
  * -infinity for its log sum.  scale 0 selects 1/sqrt(dim).
  * q: (requests, heads, dim), element (r, j, i) at r * q_row_stride +
  * j * q_head_stride + i (multiples of 8, 16-byte aligned); out: dense
@@ -124,6 +125,9 @@ B2G_API int b2g_cache_attention(const b2g_cache_attention_desc* desc, b2g_stream
  * where j <= i + m - n (the last query sees the last key).  A row that sees
  * nothing gives zeros, and -infinity for its log sum; so does a query row that
  * belongs to no sequence.
+ * What stands in another sequence never reaches a row.  Within its own, a
+ * weight of 0 is still multiplied by the value: an infinity or NaN in v also
+ * reaches earlier rows that share its tile of 128 keys.
  * q, k, v, out: element (t, h, i) at t * token_stride + h * head_stride + i,
  * strides multiples of 8 elements, 16-byte aligned; heads a multiple of
  * kv_heads, heads / kv_heads <= 128; dim a multiple of 16, at most 128.
