@@ -37,7 +37,9 @@
 // (both tiles' softmax then fall on the same cycles, +25 %), branches around
 // key columns past the diagonal (+4 %, the compiler no longer interleaves the
 // columns), O staged through shared memory for whole-line stores (-3 % where
-// items are short, +2 % where they are long).
+// items are short, +2 % where they are long), 64 keys at a time in a loop of
+// half the code (-8 % for short prompts, +5 to +19 % for long ones), P beside S
+// up to 64 dims (both softmaxes at once: +16 %).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -60,6 +62,7 @@ constexpr int kMmaWarp = 8, kLoadWarp = 9, kNextWarp = 10, kTailWarp = 11;
 constexpr int kThreads = 12 * 32;     // a whole third warpgroup, for the register split
 // Registers: 384 threads start with 168 each; the third warpgroup gives 96 of
 // each thread's to the softmax warps (2 * 128 * 216 + 128 * 72 = 384 * 168).
+// 208 / 88 was 9 % slower (a row's 128 scores no longer fit), 224 / 56 1 %.
 constexpr int kRegsSoftmax = 216, kRegsOther = 72;
 constexpr int kAskAhead = 2;          // key tiles left to load when the next item is asked for
 constexpr int kItemReaders = kSoftmaxWarps + 3;

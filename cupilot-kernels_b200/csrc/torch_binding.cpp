@@ -490,6 +490,16 @@ at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType dt, const at::Tensor& lik
   return at::detail::empty_cuda(sizes, dt, like.device(), c10::nullopt);
 }
 
+// n elements of `base`'s memory from a byte on, as a tensor of their own.
+at::Tensor part_of(const at::Tensor& base, int64_t byte, int64_t n, at::ScalarType dt) {
+  at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+      c10::Storage(base.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA),
+      c10::scalarTypeToTypeMeta(dt));
+  t.unsafeGetTensorImpl()->set_storage_offset(byte / static_cast<int64_t>(c10::elementSize(dt)));
+  t.unsafeGetTensorImpl()->set_sizes_contiguous({n});
+  return t;
+}
+
 void check_ints(const at::Tensor& t, const char* name, int64_t dims, at::ScalarType dt,
                 const at::Tensor& like) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on the same CUDA device");
@@ -566,10 +576,13 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> block_tables(const at
               "block_size must be a power of two from 16 to 256, got ", block_size);
   TORCH_CHECK(n <= B2G_MAX_TABLE_REQUESTS, "at most ", B2G_MAX_TABLE_REQUESTS, " requests");
   const c10::cuda::CUDAGuard guard(context_lens.device());
-  at::Tensor slots = fresh({total_tokens}, at::kLong, context_lens);
-  at::Tensor cu = fresh({n + 1}, at::kInt, context_lens);
-  at::Tensor lens = fresh({n}, at::kInt, context_lens);
-  at::Tensor left = fresh({1}, at::kInt, context_lens);
+  // The four results share one allocation: each of its own would be a third of the call's time.
+  const at::Tensor all = fresh({total_tokens + n + 1}, at::kLong, context_lens);
+  const int64_t ints = 8 * total_tokens;
+  at::Tensor slots = part_of(all, 0, total_tokens, at::kLong);
+  at::Tensor cu = part_of(all, ints, n + 1, at::kInt);
+  at::Tensor lens = part_of(all, ints + 4 * (n + 1), n, at::kInt);
+  at::Tensor left = part_of(all, ints + 4 * (2 * n + 1), 1, at::kInt);
   auto stream = at::cuda::getCurrentCUDAStream(context_lens.device().index());
   check_status(
       b2g_block_tables(context_lens.data_ptr<int32_t>(), new_lens.data_ptr<int32_t>(), n,
