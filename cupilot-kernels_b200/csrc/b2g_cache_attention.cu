@@ -10,7 +10,8 @@
 // share the kv head as the columns, S^T = K Q^T and O^T = V^T P^T, so that a
 // group of 8 heads fills a product.  q is brought to [-1, 1] by a power of two
 // (exact in fp16, where a row's small values may go subnormal), the weights
-// are <= 2^12 in fp16, sums, maxima and the output are fp32.
+// times their value scales are fp16 of at most 2^15, the largest of a head
+// near 2^7 (11 bits down to 2^-21 of it), sums, maxima and the output are fp32.
 //
 // Bound by memory: 2 * dim bytes a token and kv head.  A producer warp keeps
 // a ring of 64-token stages filled by TMA (boxes of whole rows of a block in
@@ -38,6 +39,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 #include <cstdint>
 
@@ -62,9 +64,13 @@ __host__ __device__ constexpr int tile_tokens(int dp, int rows) {
   return 16 * consumers(dp, rows) * pieces(dp);
 }
 constexpr float kGrow = 8.f;           // a maximum may be passed by 2^8 before the sums are rescaled
+constexpr float kLift = 7.f;           // the largest weight times value scale stands at 2^7 in fp16
 constexpr uint64_t kDrainLimitNs = 100000000ull;
 constexpr int kJoin = 4;                     // rows of parts that a joining warp loads at once
 constexpr uint32_t kNoBlock = 0xffffffffu;   // in the place of a key scale
+// What the maxima start from: below every score, yet finite, so that differences of two are no NaN.
+constexpr float kNothing = -FLT_MAX;
+constexpr float kLeastScale = -100.f;        // log2 of the least value scale that bounds the weights
 enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
 
 // Shared memory of a CTA: the ring, the stages' scales, the barriers, and the
@@ -116,6 +122,12 @@ struct Args {
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float log2_fast(float x) {
+  float y;
+  asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -177,7 +189,8 @@ struct State {
   float rf[N][2];                      // scale * log2(e) * the power of two that q was divided by
   float start[N][2];                   // what S starts from: the int8 offset's share
   float m[N][2], l[N][2];              // maximum so far (log2 units), this lane's part of the sum
-  float unit, per;                     // o is in units of `unit` (a block's value scale), per = 1 / unit
+  float b[N][2];                       // o is in units of 2^(b - m): the largest weight times value
+                                       // scale so far, over 2^kLift (log2 units)
   float o[N][DP / 16][4];              // dims DP/8 g + 2 t, + 1 (index / 2) of those heads (index % 2)
 };
 
@@ -268,59 +281,70 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
             for (int j = 0; j < DP / 32; ++j) w[x][t][j] = 0;
     }
   }
-  float top[N][2], most = fabsf(sc[0].y);
+  // Two maxima: of z for the sums l, and of z + log2 of the value scale for the
+  // weights in fp16, which then keep the bits that the output needs however
+  // far the blocks' value scales lie apart.
+  float top[N][2], tall[N][2], lg[P];
 #pragma unroll
-  for (int x = 1; x < P; ++x) most = fmaxf(most, fabsf(sc[x].y));
-  bool grow = most > 16.f * s.unit;
+  for (int x = 0; x < P; ++x) lg[x] = fmaxf(log2_fast(fabsf(sc[x].y)), kLeastScale);
+  bool grow = false;
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       top[n][h] = fmaxf(z[0][n][h], z[0][n][2 + h]);
+      tall[n][h] = top[n][h] + lg[0];
 #pragma unroll
-      for (int x = 1; x < P; ++x) top[n][h] = fmaxf(top[n][h], fmaxf(z[x][n][h], z[x][n][2 + h]));
-      grow |= top[n][h] > s.m[n][h] + kGrow;
+      for (int x = 1; x < P; ++x) {
+        const float t = fmaxf(z[x][n][h], z[x][n][2 + h]);
+        top[n][h] = fmaxf(top[n][h], t);
+        tall[n][h] = fmaxf(tall[n][h], t + lg[x]);
+      }
+      grow |= top[n][h] > s.m[n][h] + kGrow || tall[n][h] > s.b[n][h] + (kLift + kGrow);
     }
   if (__any_sync(0xffffffffu, grow)) {
-    const float unit = fmaxf(s.unit, most);
-    const float ratio = unit > 0.f ? s.unit / unit : 0.f;
 #pragma unroll
     for (int n = 0; n < N; ++n)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float t = top[n][h];
+        float t = top[n][h], b = tall[n][h];
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+        for (int o = 4; o < 32; o <<= 1) {
+          t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, o));
+          b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+        }
         t = fmaxf(t, s.m[n][h]);
-        const float corr = s.m[n][h] == -INFINITY ? 0.f : exp2_fast(s.m[n][h] - t);
+        b = fmaxf(b - kLift, s.b[n][h]);
+        s.l[n][h] *= exp2_fast(s.m[n][h] - t);
+        const float corr = exp2_fast(s.b[n][h] - b);
         s.m[n][h] = t;
-        s.l[n][h] *= corr;
+        s.b[n][h] = b;
 #pragma unroll
         for (int t16 = 0; t16 < DP / 16; ++t16) {
-          s.o[n][t16][h] *= corr * ratio;
-          s.o[n][t16][2 + h] *= corr * ratio;
+          s.o[n][t16][h] *= corr;
+          s.o[n][t16][2 + h] *= corr;
         }
       }
-    s.unit = unit;
-    s.per = unit > 0.f ? 1.f / unit : 0.f;
   }
   uint32_t p[P][N][2];
 #pragma unroll
-  for (int x = 0; x < P; ++x) {
-    const float weight = sc[x].y * s.per;
+  for (int n = 0; n < N; ++n) {
+    float per[2];
 #pragma unroll
-    for (int n = 0; n < N; ++n) {
+    for (int h = 0; h < 2; ++h) per[h] = exp2_fast(s.m[n][h] - s.b[n][h]);
+#pragma unroll
+    for (int x = 0; x < P; ++x) {
       float e[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float m = s.m[n][h] == -INFINITY ? 0.f : s.m[n][h];
-        e[h] = exp2_fast(z[x][n][h] - m);
-        e[2 + h] = exp2_fast(z[x][n][2 + h] - m);
+        e[h] = exp2_fast(z[x][n][h] - s.m[n][h]);
+        e[2 + h] = exp2_fast(z[x][n][2 + h] - s.m[n][h]);
         s.l[n][h] += e[h] + e[2 + h];
       }
+      const float weight[2] = {sc[x].y * per[0], sc[x].y * per[1]};
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const __half2 hv = __floats2half2_rn(e[2 * t] * weight, e[2 * t + 1] * weight);
+        const __half2 hv = __floats2half2_rn(e[2 * t] * weight[0], e[2 * t + 1] * weight[1]);
         p[x][n][t] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
       }
     }
@@ -634,8 +658,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) s.m[i][h] = -INFINITY, s.l[i][h] = 0.f;
-    s.unit = s.per = 0.f;
+      for (int h = 0; h < 2; ++h) s.m[i][h] = s.b[i][h] = kNothing, s.l[i][h] = 0.f;
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -676,6 +699,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
         float l = s.l[i][h];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        const float unit = exp2_fast(s.b[i][h] - s.m[i][h]);
         if (g == 0) {
           sm_m[y] = s.m[i][h];
           sm_l[y] = l;
@@ -683,8 +707,8 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
 #pragma unroll
         for (int t = 0; t < DP / 16; t += 2)
           *reinterpret_cast<float4*>(sm_o + y * DP + DP / 8 * g + 2 * t) =
-              make_float4(s.o[i][t][h] * s.unit, s.o[i][t][2 + h] * s.unit, s.o[i][t + 1][h] * s.unit,
-                          s.o[i][t + 1][2 + h] * s.unit);
+              make_float4(s.o[i][t][h] * unit, s.o[i][t][2 + h] * unit, s.o[i][t + 1][h] * unit,
+                          s.o[i][t + 1][2 + h] * unit);
       }
     asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
@@ -698,7 +722,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float wm = sm_m[w * ROWS + y];
-        const float e = wm == -INFINITY ? 0.f : exp2_fast(wm - m);
+        const float e = exp2_fast(wm - m);
         l += e * sm_l[w * ROWS + y];
         o += e * sm_o[(w * ROWS + y) * DP + d];
       }
@@ -763,8 +787,7 @@ __global__ void cache_join_kernel(const Args a) {
         const int own = base + lane * step;
         float e = 0.f;
         if (own <= c1) {
-          const float pm = a.part_m[slot_of(own)];
-          e = pm == -INFINITY ? 0.f : exp2_fast(pm - m);
+          e = exp2_fast(a.part_m[slot_of(own)] - m);
           l += e * a.part_l[slot_of(own)];
         }
         const int n = min(32, (c1 - base) / step + 1);

@@ -352,6 +352,35 @@ def test_decode_peaked_and_uneven_scales(ops, dtype):
     _decode_case(ops, [700, 33], 2, 4, 128, 16, dtype, torch.int8, seed=6, scale=0.3)
 
 
+@pytest.mark.parametrize("codes", CODES, ids=_ids)
+@pytest.mark.parametrize("power", [24, 40])
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 2), (64, 12), (128, 12)])
+def test_decode_value_scales_that_some_heads_do_not_see(ops, d, group, power, codes):
+    # Half the blocks have value scales 2^power larger; even heads weigh them with exp(-40), odd
+    # heads see little else.  The even heads' output keeps its bits, head by head.
+    g = torch.Generator().manual_seed(d + group + power)
+    # The kinds alternate every four blocks, and 150 requests share them, so that a warp meets both.
+    n, blocks, reqs = 333, 21, 150
+    sign = torch.tensor([1.0, -1.0]).repeat_interleave(4).repeat(3)[:blocks].view(blocks, 1, 1, 1)
+    kc = _codes_of(sign * 64 + torch.randint(-8, 9, (blocks, 1, 16, d), generator=g), codes)
+    vc, vs = _random_cache(g, blocks, 1, 16, d, codes)
+    ks = torch.full((blocks, 1), 1 / 64.0)
+    vs = torch.where(sign[:, :, 0, 0] < 0, vs * 2.0 ** power, vs)
+    q = torch.full((1, group, d), 20 / d ** 0.5)
+    q[:, 1::2] *= -1
+    q = q.bfloat16()
+    k, v = (c.double() * s.double()[:, :, None, None] for c, s in ((kc, ks), (vc, vs)))
+    k, v = (x.transpose(1, 2).reshape(-1, 1, d)[:n] for x in (k, v))
+    want, want_lse = _attend(q.double(), k, v, d ** -0.5)
+    out, lse = ops.cache_attention(q.cuda().repeat(reqs, 1, 1), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(),
+                                   _dev([list(range(blocks))] * reqs), _dev([n] * reqs), None, True)
+    for r in range(reqs):
+        for j in range(group):
+            _close(out[r, j], want[0, j], torch.bfloat16)
+    assert (lse.cpu().double() - want_lse).abs().max() <= LSE_TOL
+    _no_error(ops)
+
+
 def test_decode_large_queries_in_bf16(ops):
     # beyond fp16's range: q is scaled by a power of two for the products
     _decode_case(ops, [100], 1, 4, 64, 16, torch.bfloat16, torch.int8, seed=7, q_scale=1e6, scale=1e-7)
