@@ -24,12 +24,12 @@
 //
 // Measured (GB/s of codes, 6547 being the card's copy rate):
 //   64 requests of 14000 to 31000 tokens, 8 kv heads, 32 heads, dim 128, int8:
-//   465 us, 6510 GB/s; 0.53 ms once the power limit lowers the clock
+//   462 us, 6550 GB/s; 0.53 ms once the power limit lowers the clock
 //   1 request of 150001 tokens, 4 kv heads, 32 heads, e4m3: 38 us, 4070 GB/s
 //   (some 10 us are start, the cuts' partial results and their join)
 //   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 42 us,
 //   3170 GB/s (the consumers' chains of dependent products, not the loads)
-//   1 request of 997 tokens: 9.5 us, two launches and a handful of dependent
+//   1 request of 997 tokens: 8.8 us, two launches and a handful of dependent
 //   loads
 // K as the first operand instead of q halves the products (8 heads of 16 rows
 // were empty): 822 -> 475 us together with the TMA ring, whose place registers
@@ -230,21 +230,6 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
       }
     }
   }
-  // V: tokens 2c, 2c+1, 2c+8, 2c+9, dims DP/8 g ... of each.
-  uint32_t w[P][4][DP / 32];
-#pragma unroll
-  for (int x = 0; x < P; ++x)
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const int row = 16 * x + 2 * c + (t & 1) + (t >> 1) * 8;
-      if (DP == 128) {
-        const uint4 y = *reinterpret_cast<const uint4*>(v + place(row, g));
-        w[x][t][0] = y.x, w[x][t][1] = y.y, w[x][t][DP / 32 - 2] = y.z, w[x][t][DP / 32 - 1] = y.w;
-      } else {
-        const uint2 y = *reinterpret_cast<const uint2*>(v + place(row, g >> 1) + (g & 1) * 8);
-        w[x][t][0] = y.x, w[x][t][1] = y.y;
-      }
-    }
   bool part = left < 16 * P;
 #pragma unroll
   for (int x = 0; x < P; ++x) {
@@ -272,13 +257,6 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
           if (g + 8 >= here) z[x][n][2 + h] = -INFINITY;
         }
       if (here <= 0) sc[x].y = 0.f;
-      // What stands behind them may be NaN in e4m3, and 0 * NaN must not reach the sums.
-      if (E4M3)
-#pragma unroll
-        for (int t = 0; t < 4; ++t)
-          if (2 * c + (t & 1) + (t >> 1) * 8 >= here)
-#pragma unroll
-            for (int j = 0; j < DP / 32; ++j) w[x][t][j] = 0;
     }
   }
   // Two maxima: of z for the sums l, and of z + log2 of the value scale for the
@@ -349,6 +327,34 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
       }
     }
   }
+  // V: tokens 2c, 2c+1, 2c+8, 2c+9, dims DP/8 g ... of each.  Loaded here and not
+  // before the weights, which then have its registers (16 heads of 128 dims, int8: 67.2 -> 64.8 us
+  // at 16 requests of 10000 tokens; 8 heads: 63.8 -> 62.1).
+  uint32_t w[P][4][DP / 32];
+#pragma unroll
+  for (int x = 0; x < P; ++x)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int row = 16 * x + 2 * c + (t & 1) + (t >> 1) * 8;
+      if (DP == 128) {
+        const uint4 y = *reinterpret_cast<const uint4*>(v + place(row, g));
+        w[x][t][0] = y.x, w[x][t][1] = y.y, w[x][t][DP / 32 - 2] = y.z, w[x][t][DP / 32 - 1] = y.w;
+      } else {
+        const uint2 y = *reinterpret_cast<const uint2*>(v + place(row, g >> 1) + (g & 1) * 8);
+        w[x][t][0] = y.x, w[x][t][1] = y.y;
+      }
+    }
+  // What stands behind the last token may be NaN in e4m3, and 0 * NaN must not reach the sums.
+  if (E4M3 && part)
+#pragma unroll
+    for (int x = 0; x < P; ++x) {
+      const int here = __float_as_uint(sc[x].x) == kNoBlock ? 0 : left - 16 * x;
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+        if (2 * c + (t & 1) + (t >> 1) * 8 >= here)
+#pragma unroll
+          for (int j = 0; j < DP / 32; ++j) w[x][t][j] = 0;
+    }
 #pragma unroll
   for (int x = 0; x < P; ++x)
 #pragma unroll
