@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const TableArgs a
           block = *entry;
         } else {
           const int64_t at = count - 1 - (first[lo] + j - held);
-          block = at >= 0 ? a.free_blocks[at] : -1;
+          block = at >= 0 && at < count ? a.free_blocks[at] : -1;
           if (off == 0) *entry = static_cast<int32_t>(block);
         }
         if (block >= 0) slot = (block << a.lg_block) + off;
