@@ -65,6 +65,11 @@ class PagedCache:
     def _held(self, tokens: int) -> int:
         return -(-tokens // self.block_size)
 
+    def _open(self) -> Step:
+        if self.step is None:
+            raise RuntimeError("begin() opens a step first")
+        return self.step
+
     def begin(self, new_lens: Sequence[int]) -> Step:
         """Make room for `new_lens[r]` more tokens of each request r."""
         new_lens = [int(n) for n in new_lens]
@@ -89,25 +94,24 @@ class PagedCache:
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Keep the step's keys and values (tokens, kv_heads, dim)."""
-        if self.step is None:
-            raise RuntimeError("begin() opens a step first")
-        ops.cache_append(k, v, self.step.slots, self.k_cache[layer], self.v_cache[layer],
+        ops.cache_append(k, v, self._open().slots, self.k_cache[layer], self.v_cache[layer],
                          self.k_scale[layer], self.v_scale[layer])
 
     def prefill(self, layer: int, q, k, v, scale=None) -> torch.Tensor:
         """The step's prompts: keep their keys and values, and attend to them."""
-        self.append(layer, k, v)
-        if any(n and c for n, c in zip(self.step.new_lens, self.step.contexts)):
+        step = self._open()
+        if any(n and c for n, c in zip(step.new_lens, step.contexts)):
             raise RuntimeError("prefill() is for requests that held no token")
+        self.append(layer, k, v)
         return ops.prompt_attention(q, k, v, self.step.cu_seqlens, scale=scale)
 
     def decode(self, layer: int, q, k, v, scale=None) -> torch.Tensor:
         """One token of each request that gains one: keep its key and value, and attend to all
         that the request holds."""
-        self.append(layer, k, v)
-        new_lens = self.step.new_lens
+        new_lens = self._open().new_lens
         if max(new_lens) > 1:
             raise RuntimeError("decode() is for steps of one token a request")
+        self.append(layer, k, v)
         table, lens = self.block_table, self.step.seq_lens
         if min(new_lens) == 0:
             rows = torch.tensor([r for r, n in enumerate(new_lens) if n], pin_memory=True).to(
@@ -118,6 +122,8 @@ class PagedCache:
 
     def release(self, request: int) -> None:
         """Give a finished request's blocks back; its row is free for another."""
+        if not 0 <= request < len(self.lengths):
+            raise IndexError(f"request must be from 0 to {len(self.lengths) - 1}, got {request}")
         n = self._held(self.lengths[request])
         self.free_blocks[self.free:self.free + n] = self.block_table[request, :n]
         self.free += n

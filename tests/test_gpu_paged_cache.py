@@ -83,3 +83,28 @@ def test_refusals(serving):
         serving.PagedCache(1, 1, 16, 1, 1, 20)
     with pytest.raises(ValueError, match="block_size"):
         serving.PagedCache(1, 1, 16, 1, 1, 16, block_size=24)
+
+
+@pytest.mark.parametrize("request_", [-1, 2])
+def test_release_of_a_request_that_is_not_there(serving, request_):
+    c = serving.PagedCache(layers=1, requests=2, max_tokens=64, blocks=4, kv_heads=1, dim=16)
+    c.begin([16, 16])
+    with pytest.raises(IndexError, match="from 0 to 1"):
+        c.release(request_)
+    assert c.free == 2 and c.lengths == [16, 16] and c.lens.tolist() == [16, 16]
+    assert c.free_count.item() == 2
+
+
+def test_refused_steps_leave_the_cache_as_it_was(serving):
+    c = serving.PagedCache(layers=1, requests=2, max_tokens=64, blocks=4, kv_heads=1, dim=16)
+    x = torch.ones(3, 1, 16, device="cuda").half()
+    for call in (c.prefill, c.decode):
+        with pytest.raises(RuntimeError, match="begin"):
+            call(0, x, x, x)
+    c.begin([3, 0])
+    with pytest.raises(RuntimeError, match="one token a request"):
+        c.decode(0, x, x, x)
+    c.begin([3, 0])
+    with pytest.raises(RuntimeError, match="held no token"):
+        c.prefill(0, x, x, x)
+    assert (c.k_cache.view(torch.uint8) == 0).all() and (c.v_scale == 0).all()
