@@ -516,7 +516,7 @@ at::Tensor rows_of(const at::Tensor& t) {
   for (int i = 0; i < 2; ++i)
     if (t.size(i) > 1 && (t.stride(i) <= 0 || t.stride(i) % 8)) fine = false;
   if (reinterpret_cast<uintptr_t>(t.data_ptr()) % 16) fine = false;
-  return fine ? t : t.contiguous();
+  return fine ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 // A stride that is never stepped may hold anything: make it one the kernels take.
 int64_t stride_of(const at::Tensor& t, int i) {

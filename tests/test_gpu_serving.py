@@ -782,3 +782,27 @@ def test_empty_calls(ops):
     none = torch.zeros(0, 2, 16, 64, dtype=torch.int8, device="cuda")
     out = ops.cache_attention(q, none, none, ks[:0], ks[:0], _dev([[0], [0]]), _dev([3, 0]))
     assert (out == 0).all()
+
+
+def test_rows_that_begin_off_16_bytes(ops):
+    # dense, so that a dense copy is what it is already
+    g = torch.Generator().manual_seed(70)
+
+    def odd(*shape):
+        n = math.prod(shape)
+        return torch.randn(n + 1, generator=g).half().cuda()[1:].view(shape)
+
+    q, k, v = odd(20, 4, 64), odd(20, 2, 64), odd(20, 2, 64)
+    cu = _dev([0, 7, 20])
+    assert torch.equal(ops.prompt_attention(q, k, v, cu), ops.prompt_attention(q.clone(), k.clone(), v.clone(), cu))
+    caches = []
+    for a, b in ((k, v), (k.clone(), v.clone())):
+        c = [torch.zeros(2, 2, 16, 64, dtype=torch.int8, device="cuda") for _ in range(2)]
+        c += [torch.zeros(2, 2, device="cuda") for _ in range(2)]
+        ops.cache_append(a, b, torch.arange(20, device="cuda"), *c)
+        caches.append(c)
+    assert all(torch.equal(x, y) for x, y in zip(*caches))
+    table, lens = _dev([[0, 1]]), _dev([20])
+    assert torch.equal(ops.cache_attention(q[:1], *caches[0], table, lens),
+                       ops.cache_attention(q[:1].clone(), *caches[0], table, lens))
+    _no_error(ops)
