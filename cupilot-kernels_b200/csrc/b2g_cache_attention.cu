@@ -14,11 +14,11 @@
 // near 2^7 (11 bits down to 2^-21 of it), sums, maxima and the output are fp32.
 //
 // Bound by memory: 2 * dim bytes a token and kv head.  A producer warp keeps
-// a ring of 64-token stages filled by TMA (boxes of whole rows of a block in
-// the 128-byte swizzle, which the fragments' 16-byte shared loads read
-// without bank conflicts), with the blocks' scales beside them; four consumer
-// warps take 16 tokens each of every stage.  The (request, head, 64-token)
-// tiles are laid end to end and cut into equal ranges, one a CTA, so ragged
+// a ring of stages of 64 to 128 tokens filled by TMA (boxes of whole rows of a
+// block in the 128-byte or 64-byte swizzle, which the fragments' shared loads
+// read without bank conflicts), with the blocks' scales beside them; four or
+// five consumer warps take 16 or 32 tokens each of every stage.  The (request,
+// head, stage) tiles are laid end to end and cut into equal ranges, one a CTA, so ragged
 // lengths fill the GPU evenly; what a cut divides is joined by a second small
 // kernel.
 //
@@ -27,8 +27,8 @@
 //   462 us, 6550 GB/s; 0.53 ms once the power limit lowers the clock
 //   1 request of 150001 tokens, 4 kv heads, 32 heads, e4m3: 38 us, 4070 GB/s
 //   (some 10 us are start, the cuts' partial results and their join)
-//   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 42 us,
-//   3170 GB/s (the consumers' chains of dependent products, not the loads)
+//   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 39 us,
+//   3370 GB/s (the consumers' chains of dependent products, not the loads)
 //   1 request of 997 tokens: 8.8 us, two launches and a handful of dependent
 //   loads
 // K as the first operand instead of q halves the products (8 heads of 16 rows
@@ -77,7 +77,12 @@ enum : int { kErrFull = 0x311, kErrEmpty = 0x312 };
 // four warps' results of a segment.
 template <int DP, int ROWS>
 struct Smem {
-  static constexpr int kStages = 3;
+  // Multiprocessor's CTAs and their stages: with rows of 64 bytes and 8 heads the products' chains
+  // want a fourth CTA's warps more than the ring its third stage (64 requests of 20000 tokens, int8:
+  // 247 -> 226 us; 48 ragged ones: 41.7 -> 39.3).
+  static constexpr bool kFour = DP == 64 && ROWS == 8;
+  static constexpr int kCtas = kFour ? 4 : ROWS == 8 ? 3 : 2;
+  static constexpr int kStages = kFour ? 2 : 3;
   static constexpr int kWarps = consumers(DP, ROWS), kThreads = (kWarps + 1) * 32;
   static constexpr int kTile = tile_tokens(DP, ROWS);
   static constexpr int kPieces = kTile / 16;
@@ -89,7 +94,6 @@ struct Smem {
   static constexpr int kOffJoin = (kOffMisc + 64 + 15) / 16 * 16;   // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
   static constexpr int kOffO = kOffJoin + 2 * kWarps * ROWS * 4;
   static constexpr int kBytes = kOffO + kWarps * ROWS * DP * 4 + 1024;
-  static constexpr int kCtas = ROWS == 8 ? 3 : 2;           // a multiprocessor
   static_assert(kSideBytes % 1024 == 0 && kOffScales % 8 == 0 && kOffBars % 8 == 0 && kOffO % 16 == 0,
                 "swizzle atoms, float2 scales, barriers, float4 sums");
   static_assert(kCtas * (kBytes + 1024) <= 227 * 1024 + 1024, "shared memory of an SM");
@@ -648,7 +652,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
   uint32_t n = 0;
   bool first = true;
   // With rows of 64 bytes the next segment's queries are fetched before this one is joined (48
-  // ragged requests: 44.3 -> 42.2 us); with 128 the registers for it are not there (60.5 -> 64.0).
+  // ragged requests: 44.3 -> 42.2 us when it was taken); with 128 the registers for it are not there (60.5 -> 64.0).
   constexpr bool kAhead = DP == 64;
   uint4 raw[N][DP / 32];
   auto fetch = [&]() {
@@ -869,8 +873,9 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   w.row_groups = static_cast<int>(cdiv(group, w.rows));
   const int64_t most = d->requests * d->kv_heads * w.row_groups *
                        std::max<int64_t>(cdiv(d->table_width * d->block_size, tile_tokens(w.dp, w.rows)), 1);
-  w.grid = static_cast<int>(std::min<int64_t>(
-      std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * (w.rows == 8 ? Smem<128, 8>::kCtas : Smem<128, 16>::kCtas)));
+  const int ctas = w.dp == 64 ? (w.rows == 8 ? Smem<64, 8>::kCtas : Smem<64, 16>::kCtas)
+                              : (w.rows == 8 ? Smem<128, 8>::kCtas : Smem<128, 16>::kCtas);
+  w.grid = static_cast<int>(std::min<int64_t>(std::max<int64_t>(most, 1), static_cast<int64_t>(sms) * ctas));
   auto pad = [](int64_t n) { return cdiv(n, 256) * 256; };
   w.off_m = pad((d->requests + 1) * 4);
   w.off_l = w.off_m + pad(2ll * w.grid * w.rows * 4);
