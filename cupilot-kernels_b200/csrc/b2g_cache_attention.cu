@@ -93,8 +93,8 @@ struct Smem {
   static constexpr int kOffScales = kStages * kStageBytes;  // [stage][piece]{k scale, v scale}
   static constexpr int kOffBars = kOffScales + kStages * kPieces * 8;
   static constexpr int kOffMisc = kOffBars + 2 * kStages * 8;
-  static constexpr int kOffJoin = (kOffMisc + 64 + 15) / 16 * 16;   // m, l: [warp][ROWS]; o: [warp][ROWS][DP]
-  static constexpr int kOffO = kOffJoin + 2 * kWarps * ROWS * 4;
+  static constexpr int kOffJoin = (kOffMisc + 64 + 15) / 16 * 16;   // m, l, b: [warp][ROWS]; o: [warp][ROWS][DP]
+  static constexpr int kOffO = kOffJoin + 3 * kWarps * ROWS * 4;
   static constexpr int kBytes = kOffO + kWarps * ROWS * DP * 4 + 1024;
   static_assert(kSideBytes % 1024 == 0 && kOffScales % 8 == 0 && kOffBars % 8 == 0 && kOffO % 16 == 0,
                 "swizzle atoms, float2 scales, barriers, float4 sums");
@@ -119,6 +119,7 @@ struct Args {
   int* prefix;
   float* part_m;
   float* part_l;
+  float* part_b;
   float* part_o;
   int grid;
   long long wait_limit_ns;
@@ -195,8 +196,8 @@ struct State {
   float rf[N][2];                      // scale * log2(e) * the power of two that q was divided by
   float start[N][2];                   // what S starts from: the int8 offset's share
   float m[N][2], l[N][2];              // maximum so far (log2 units), this lane's part of the sum
-  float b[N][2];                       // o is in units of 2^(b - m): the largest weight times value
-                                       // scale so far, over 2^kLift (log2 units)
+  float b[N][2];                       // o is in units of 2^b, l in units of 2^m: b is the largest of
+                                       // z + log2(value scale) so far, less kLift
   float o[N][DP / 16][4];              // dims DP/8 g + 2 t, + 1 (index / 2) of those heads (index % 2)
 };
 
@@ -310,25 +311,24 @@ __device__ __forceinline__ void compute_pieces(State<DP, ROWS>& s, const uint8_t
         }
       }
   }
+  // The weight in fp16 is 2^(z - b) times the value scale, of at most 2^(kLift + kGrow) by the test
+  // above.  2^(z - b) alone stays finite too (b takes no scale for less than 2^kLeastScale); a factor
+  // 2^(m - b) in its place would not beside a larger scale: where blocks of zeros lead, b lies 107 below m.
   uint32_t p[P][N][2];
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    float per[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) per[h] = exp2_fast(s.m[n][h] - s.b[n][h]);
 #pragma unroll
     for (int x = 0; x < P; ++x) {
-      float e[4];
+      float w[4];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        e[h] = exp2_fast(z[x][n][h] - s.m[n][h]);
-        e[2 + h] = exp2_fast(z[x][n][2 + h] - s.m[n][h]);
-        s.l[n][h] += e[h] + e[2 + h];
+        s.l[n][h] += exp2_fast(z[x][n][h] - s.m[n][h]) + exp2_fast(z[x][n][2 + h] - s.m[n][h]);
+        w[h] = exp2_fast(z[x][n][h] - s.b[n][h]) * sc[x].y;
+        w[2 + h] = exp2_fast(z[x][n][2 + h] - s.b[n][h]) * sc[x].y;
       }
-      const float weight[2] = {sc[x].y * per[0], sc[x].y * per[1]};
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
-        const __half2 hv = __floats2half2_rn(e[2 * t] * weight[0], e[2 * t + 1] * weight[1]);
+        const __half2 hv = __floats2half2_rn(w[2 * t], w[2 * t + 1]);
         p[x][n][t] = transpose8x8(*reinterpret_cast<const uint32_t*>(&hv));
       }
     }
@@ -454,6 +454,13 @@ __device__ __forceinline__ void store_out(const Args& a, int64_t at, float v) {
     static_cast<__half*>(a.out)[at] = __float2half_rn(v);
 }
 
+// o 2^shift / l; zeros where no token was seen, NaN where the sum is NaN.  The
+// power in two steps: it alone may pass fp32's range, the result not.
+__device__ __forceinline__ float quotient(float o, float shift, float l) {
+  const float half = exp2_fast(0.5f * shift);
+  return l > 0.f ? o * half / l * half : (l == 0.f ? 0.f : l);
+}
+
 // Tiles before each request: every thread sums a run of requests, the runs'
 // sums are scanned.  Returns the total; *run is the sum before this thread's
 // run, *lo and *hi the run.
@@ -532,6 +539,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
   int* start = misc + 8;                 // request, tiles before it
   float* sm_m = reinterpret_cast<float*>(smem + L::kOffJoin);
   float* sm_l = sm_m + kWarps * ROWS;
+  float* sm_b = sm_l + kWarps * ROWS;
   float* sm_o = reinterpret_cast<float*>(smem + L::kOffO);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   ptx::griddep_launch_dependents();
@@ -702,7 +710,8 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
     more = seg.next(a);
     if (more && kAhead) fetch();
 
-    // Join the warps.
+    // Join the warps.  Sums and outputs keep their own units, 2^m and 2^b, through both joins: 2^(b - m)
+    // has no place in 32 bits where blocks that weigh nothing lead by 2^126.
 #pragma unroll
     for (int i = 0; i < N; ++i)
 #pragma unroll
@@ -711,43 +720,54 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
         float l = s.l[i][h];
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        const float unit = exp2_fast(s.b[i][h] - s.m[i][h]);
         if (g == 0) {
           sm_m[y] = s.m[i][h];
           sm_l[y] = l;
+          sm_b[y] = s.b[i][h];
         }
 #pragma unroll
         for (int t = 0; t < DP / 16; t += 2)
           *reinterpret_cast<float4*>(sm_o + y * DP + DP / 8 * g + 2 * t) =
-              make_float4(s.o[i][t][h] * unit, s.o[i][t][2 + h] * unit, s.o[i][t + 1][h] * unit,
-                          s.o[i][t + 1][2 + h] * unit);
+              make_float4(s.o[i][t][h], s.o[i][t][2 + h], s.o[i][t + 1][h], s.o[i][t + 1][2 + h]);
       }
     asm volatile("bar.sync 1, %0;" ::"n"(kWarps * 32) : "memory");
     const int64_t slot = 2 * static_cast<int64_t>(blockIdx.x) + (first ? 0 : 1);
     const int rows = min(ROWS, a.group - rg * ROWS);
-    for (int i = tid; i < rows * DP; i += kWarps * 32) {
-      const int y = i / DP, d = i % DP;
-      float m = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) m = fmaxf(m, sm_m[w * ROWS + y]);
-      float l = 0.f, o = 0.f;
+    // Four dims a thread (2 x, 2 x + 1 and those DP / 2 behind): the units' powers once for all of them.
+    for (int i = tid; i < rows * (DP / 4); i += kWarps * 32) {
+      const int y = i / (DP / 4), d = 2 * (i % (DP / 4));
+      float m = -INFINITY, b = -INFINITY;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float wm = sm_m[w * ROWS + y];
-        const float e = exp2_fast(wm - m);
-        l += e * sm_l[w * ROWS + y];
-        o += e * sm_o[(w * ROWS + y) * DP + d];
+        m = fmaxf(m, sm_m[w * ROWS + y]);
+        b = fmaxf(b, sm_b[w * ROWS + y]);
+      }
+      float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float e = exp2_fast(sm_b[w * ROWS + y] - b);
+        l += exp2_fast(sm_m[w * ROWS + y] - m) * sm_l[w * ROWS + y];
+        const float2* from = reinterpret_cast<const float2*>(sm_o + (w * ROWS + y) * DP + d);
+        const float2 lo = from[0], hi = from[DP / 4];
+        o[0] += e * lo.x, o[1] += e * lo.y, o[2] += e * hi.x, o[3] += e * hi.y;
       }
       if (whole) {
         const int64_t j =
             static_cast<int64_t>(r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
-        if (d < a.dim) store_out(a, j * a.dim + d, l > 0.f ? o / l : (l == 0.f ? 0.f : l));
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const int at = d + (x & 1) + (x >> 1) * (DP / 2);
+          if (at < a.dim) store_out(a, j * a.dim + at, quotient(o[x], b - m, l));
+        }
         if (d == 0 && a.lse) a.lse[j] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
       } else {
-        a.part_o[(slot * ROWS + y) * DP + d] = o;
+        float2* to = reinterpret_cast<float2*>(a.part_o + (slot * ROWS + y) * DP + d);
+        to[0] = make_float2(o[0], o[1]);
+        to[DP / 4] = make_float2(o[2], o[3]);
         if (d == 0) {
           a.part_m[slot * ROWS + y] = m;
           a.part_l[slot * ROWS + y] = l;
+          a.part_b[slot * ROWS + y] = b;
         }
       }
     }
@@ -787,20 +807,26 @@ __global__ void cache_join_kernel(const Args a) {
   for (int y = SPREAD ? last_row - 1 : warp; y < last_row; y += SPREAD ? ROWS : warps) {
     const int64_t at = static_cast<int64_t>(r) * a.kv_heads * a.group + head * a.group + rg * ROWS + y;
     auto slot_of = [&](int c) { return (2ll * c + (c == c0 && late ? 1 : 0)) * ROWS + y; };
-    float m = -INFINITY, l = 0.f, acc[DP / 32];
+    float m = -INFINITY, b = -INFINITY, l = 0.f, acc[DP / 32];
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) acc[i] = 0.f;
     if (tiles > 0) {
-      for (int c = c0 + lane; c <= c1; c += 32) m = fmaxf(m, a.part_m[slot_of(c)]);
+      for (int c = c0 + lane; c <= c1; c += 32) {
+        m = fmaxf(m, a.part_m[slot_of(c)]);
+        b = fmaxf(b, a.part_b[slot_of(c)]);
+      }
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+      for (int o = 16; o > 0; o >>= 1) {
+        m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, o));
+      }
       // A warp's parts: their weights side by side in the lanes, their rows kJoin at a time.
       for (int base = c0 + first; base <= c1; base += 32 * step) {
         const int own = base + lane * step;
         float e = 0.f;
         if (own <= c1) {
-          e = exp2_fast(a.part_m[slot_of(own)] - m);
-          l += e * a.part_l[slot_of(own)];
+          e = exp2_fast(a.part_b[slot_of(own)] - b);
+          l += exp2_fast(a.part_m[slot_of(own)] - m) * a.part_l[slot_of(own)];
         }
         const int n = min(32, (c1 - base) / step + 1);
         for (int k = 0; k < n; k += kJoin) {
@@ -841,7 +867,7 @@ __global__ void cache_join_kernel(const Args a) {
 #pragma unroll
     for (int i = 0; i < DP / 32; ++i) {
       const int d = lane + 32 * i;
-      if (d < a.dim) store_out(a, at * a.dim + d, l > 0.f ? acc[i] / l : (l == 0.f ? 0.f : l));
+      if (d < a.dim) store_out(a, at * a.dim + d, quotient(acc[i], b - m, l));
     }
     if (lane == 0 && a.lse) a.lse[at] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
   }
@@ -864,7 +890,7 @@ int check(const b2g_cache_attention_desc* d) {
 
 struct Layout {
   int rows, dp, row_groups, grid;
-  int64_t off_m, off_l, off_o, bytes;
+  int64_t off_m, off_l, off_b, off_o, bytes;
 };
 
 Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
@@ -881,7 +907,8 @@ Layout layout_of(const b2g_cache_attention_desc* d, int sms) {
   auto pad = [](int64_t n) { return cdiv(n, 256) * 256; };
   w.off_m = pad((d->requests + 1) * 4);
   w.off_l = w.off_m + pad(2ll * w.grid * w.rows * 4);
-  w.off_o = w.off_l + pad(2ll * w.grid * w.rows * 4);
+  w.off_b = w.off_l + pad(2ll * w.grid * w.rows * 4);
+  w.off_o = w.off_b + pad(2ll * w.grid * w.rows * 4);
   w.bytes = w.off_o + 2ll * w.grid * w.rows * w.dp * 4;
   return w;
 }
@@ -990,6 +1017,7 @@ extern "C" int b2g_cache_attention(const b2g_cache_attention_desc* d, b2g_stream
   a.prefix = reinterpret_cast<int*>(ws);
   a.part_m = reinterpret_cast<float*>(ws + w.off_m);
   a.part_l = reinterpret_cast<float*>(ws + w.off_l);
+  a.part_b = reinterpret_cast<float*>(ws + w.off_b);
   a.part_o = reinterpret_cast<float*>(ws + w.off_o);
   a.grid = w.grid;
   a.wait_limit_ns = b2g::current_wait_limit_ns();

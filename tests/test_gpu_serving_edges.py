@@ -1,0 +1,42 @@
+"""Edges of the serving operators: inputs at which a range, a limit or a mask
+decides (include/b2g_serving.h), against plain implementations in 64 bits.
+Tolerances as in test_gpu_serving.py where none is stated beside the test.
+"""
+import math
+
+import pytest
+import torch
+
+from test_gpu_serving import CODES, DTYPES, _attend, _close, _codes_of, _dev, _ids, _no_error, _random_cache
+
+pytestmark = pytest.mark.gpu
+
+
+# ------------------------------------------- cache attention: value scales
+@pytest.mark.parametrize("codes", CODES, ids=_ids)
+@pytest.mark.parametrize("gap,power", [(120, 28), (200, 28), (130, 110)])
+@pytest.mark.parametrize("d,group", [(64, 2), (128, 2), (64, 12), (128, 12)])
+def test_blocks_of_zeros_lead_before_large_value_scales(ops, d, group, gap, power, codes):
+    """The first blocks lead by 2^gap and hold zeros only (value scale 0); the later ones, with value
+    scales of 2^power, are then all of the output: finite, and in range at (130, 110)."""
+    g = torch.Generator().manual_seed(d + group + gap)
+    # 700 requests share the blocks, so that one warp meets both kinds.
+    n, zeros, blocks, reqs = 333, 10, 21, 700
+    lead = (torch.arange(blocks) < zeros).view(blocks, 1)
+    sign = torch.where(lead, 1.0, -1.0)[:, :, None, None]
+    kc = _codes_of(sign * 64 + torch.randint(-8, 9, (blocks, 1, 16, d), generator=g), codes)
+    vc, vs = _random_cache(g, blocks, 1, 16, d, codes)
+    ks = torch.full((blocks, 1), 1 / 64.0)
+    vs = torch.where(lead, 0.0, vs * 2.0 ** power)
+    vc = torch.where(lead[:, :, None, None], 0, vc.view(torch.uint8)).view(codes)
+    q = torch.full((1, group, d), gap / 2 * math.log(2.0) / d ** 0.5).bfloat16()
+    k, v = (c.double() * s.double()[:, :, None, None] for c, s in ((kc, ks), (vc, vs)))
+    k, v = (x.transpose(1, 2).reshape(-1, 1, d)[:n] for x in (k, v))
+    want, _ = _attend(q.double(), k, v, d ** -0.5)
+    want = want.bfloat16().double()              # (2^-172 at gap 200: 0)
+    out = ops.cache_attention(q.cuda().repeat(reqs, 1, 1), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(),
+                              _dev([list(range(blocks))] * reqs), _dev([n] * reqs))
+    assert torch.isfinite(out).all()
+    for j in range(group):
+        _close(out[:, j], want[:, j].expand(reqs, d), torch.bfloat16)
+    _no_error(ops)
