@@ -220,13 +220,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // 2^x of a pair by range reduction and a polynomial: x = n + f, |f| <= 1/2,
 // 2^f by its best relative approximation of degree 3 (error 7.5e-5, for P in
 // bf16 with its rounding of 2e-3) or 4 (2.6e-6, for fp16 with 2.4e-4), the
-// coefficients found by Remez exchange; n goes into the exponent.  Below
-// 2^-126 it stays there, which is nothing beside the row's maximum.
+// coefficients found by Remez exchange; n goes into the exponent.  From -127
+// on the result is 0: a masked score, -infinity, has to weigh nothing beside
+// the largest values that bf16 holds (2^-126 of those is 4).
 template <bool BF16>
 __device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
   float x, y;
   unpair(x2, x, y);
-  x2 = pair(fmaxf(x, -126.f), fmaxf(y, -126.f));
+  x2 = pair(fmaxf(x, -127.f), fmaxf(y, -127.f));
   const float big = 12582912.f;                     // 1.5 * 2^23: the sum's low bits are n
   const uint64_t n2 = add2(x2, pair(big, big));
   const uint64_t back = add2(n2, pair(-big, -big));
@@ -245,8 +246,9 @@ __device__ __forceinline__ void exp2_poly(uint64_t x2, float& a, float& b) {
   float na, nb;
   unpair(n2, na, nb);
   unpair(y2, a, b);
-  a = __uint_as_float(__float_as_uint(a) + (__float_as_uint(na) << 23));
-  b = __uint_as_float(__float_as_uint(b) + (__float_as_uint(nb) << 23));
+  // 2^f is just below 1 at f = 0, so that the sum is negative there for n = -127.
+  a = __int_as_float(max(static_cast<int>(__float_as_uint(a) + (__float_as_uint(na) << 23)), 0));
+  b = __int_as_float(max(static_cast<int>(__float_as_uint(b) + (__float_as_uint(nb) << 23)), 0));
 }
 
 // Two tiles of one sequence and kv head; all lengths cut to the tensors' sizes.

@@ -40,3 +40,21 @@ def test_blocks_of_zeros_lead_before_large_value_scales(ops, d, group, gap, powe
     for j in range(group):
         _close(out[:, j], want[:, j].expand(reqs, d), torch.bfloat16)
     _no_error(ops)
+
+
+# ---------------------------------------------- prompts: values not yet seen
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("h,d", [(1, 64), (1, 128), (60, 64)])
+def test_later_values_near_the_types_end_do_not_reach_earlier_rows(ops, h, d, dtype):
+    """A masked weight is 0: the largest finite values behind a row change no bit of it."""
+    g = torch.Generator().manual_seed(h + d)
+    n = 300
+    q, k, v = (torch.randn(n, h, d, generator=g).to(dtype).cuda() for _ in range(3))
+    cu = _dev([0, n])
+    want, lse = ops.prompt_attention(q, k, v, cu, return_lse=True)
+    for row in (1, 9, 10, 21, 31, 127, 128, 200, 299):
+        big = v.clone()
+        big[row:] = torch.finfo(dtype).max
+        got, got_lse = ops.prompt_attention(q, k, big, cu, return_lse=True)
+        assert torch.equal(got[:row], want[:row])
+        assert torch.equal(got_lse, lse)
