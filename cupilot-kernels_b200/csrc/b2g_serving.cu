@@ -35,6 +35,8 @@ int log2_of(int64_t x) {
 // one dependent load of the block, one store (8 requests: 2.5 us; 1000
 // requests with 64000 new tokens: 4.9 us).
 
+constexpr int64_t kSmallStep = 256;   // requests of a step that the smaller CTAs take
+
 struct TableArgs {
   const int32_t* context_lens;
   const int32_t* new_lens;
@@ -398,13 +400,21 @@ extern "C" int b2g_block_tables(const int32_t* context_lens, const int32_t* new_
   const size_t bytes = (3 * requests + 1) * sizeof(int);
   // Fewer threads start a small step sooner (8 requests: 2.4 us for 2.9), more scan a large one in
   // fewer rounds.
-  const bool small = requests <= 256;
+  const bool small = requests <= kSmallStep;
   const int threads = small ? 256 : 512;
   auto* kernel = small ? block_tables_kernel<256> : block_tables_kernel<512>;
-  if (bytes > 48 * 1024 &&
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                           static_cast<int>(bytes)) != cudaSuccess)
-    return B2G_ERR_LAUNCH;
+  // The larger kernel may take what the largest step needs, whatever this one does: a limit that
+  // followed the calls could be lowered between another thread's setting and its launch.
+  static thread_local int configured = -1;
+  int device = 0;
+  cudaGetDevice(&device);
+  if (!small && configured != device) {
+    constexpr int kMost = (3 * B2G_MAX_TABLE_REQUESTS + 1) * sizeof(int);
+    if (cudaFuncSetAttribute(block_tables_kernel<512>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             kMost) != cudaSuccess)
+      return B2G_ERR_LAUNCH;
+    configured = device;
+  }
   const int grid = static_cast<int>(
       std::min<int64_t>(std::max<int64_t>(cdiv(total_tokens, threads), 1), dev.num_sms));
   kernel<<<grid, threads, bytes, static_cast<cudaStream_t>(stream_handle)>>>(a);

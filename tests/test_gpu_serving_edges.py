@@ -3,10 +3,13 @@ decides (include/b2g_serving.h), against plain implementations in 64 bits.
 Tolerances as in test_gpu_serving.py where none is stated beside the test.
 """
 import math
+import subprocess
+import sys
 
 import pytest
 import torch
 
+from conftest import REPO
 from test_gpu_serving import CODES, DTYPES, _attend, _close, _codes_of, _dev, _ids, _no_error, _random_cache
 
 pytestmark = pytest.mark.gpu
@@ -58,3 +61,36 @@ def test_later_values_near_the_types_end_do_not_reach_earlier_rows(ops, h, d, dt
         got, got_lse = ops.prompt_attention(q, k, big, cu, return_lse=True)
         assert torch.equal(got[:row], want[:row])
         assert torch.equal(got_lse, lse)
+
+
+# ------------------------------------------------ block tables: their limits
+_ONE_TOKEN_EACH = """
+import importlib, torch
+ops = importlib.import_module("cupilot-kernels_b200.ops")
+n = {n}
+ctx = torch.arange(n, dtype=torch.int32, device="cuda") % 40
+table = torch.arange(3 * n, dtype=torch.int32, device="cuda").view(n, 3)
+free = 3 * n + torch.arange(n, dtype=torch.int32, device="cuda")
+new = torch.ones(n, dtype=torch.int32, device="cuda")
+count = torch.full((1,), n, dtype=torch.int32, device="cuda")
+slots, cu, lens, left = ops.block_tables(ctx, new, table, free, count, n, 16)
+opens = ctx % 16 == 0
+at = n - 1 - (opens.int().cumsum(0) - opens.int())
+block = torch.where(opens, free[at], table.gather(1, (ctx // 16).long()[:, None])[:, 0])
+assert torch.equal(slots, block.long() * 16 + ctx % 16)
+assert torch.equal(cu, torch.arange(n + 1, dtype=torch.int32, device="cuda"))
+assert torch.equal(lens, ctx + 1) and left.item() == n - opens.sum().item()
+assert ops.read_device_error(0) == 0
+"""
+
+
+@pytest.mark.parametrize("n", [4085, 4086, 4095, 4096, 16384])
+def test_tables_of_many_requests(ops, n):
+    exec(_ONE_TOKEN_EACH.format(n=n), {})
+
+
+def test_tables_of_4086_requests_first_in_a_process():
+    # 48 KB of shared memory together with the kernel's own 128 bytes; no larger call came before
+    code = f"import sys\nsys.path.insert(0, {str(REPO)!r})" + _ONE_TOKEN_EACH.format(n=4086)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]
