@@ -16,7 +16,7 @@ tokens that follow.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import List, Sequence
+from typing import List, Optional, Sequence, Tuple
 
 import torch
 
@@ -33,6 +33,8 @@ class Step:
     slots: torch.Tensor            # each new token's place in the cache
     cu_seqlens: torch.Tensor       # new tokens before each request
     seq_lens: torch.Tensor         # tokens after the step
+    # Where some requests gain one token and the others none: the former's table rows and lengths.
+    gaining: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
 
 
 class PagedCache:
@@ -87,7 +89,12 @@ class PagedCache:
             self.lens.device, non_blocking=True)
         slots, cu, lens, left = ops.block_tables(self.lens, gained, self.block_table, self.free_blocks,
                                                  self.free_count, sum(new_lens), self.block_size)
-        self.step = Step(new_lens, self.lengths, slots, cu, lens)
+        gaining = None
+        if min(new_lens) == 0 and max(new_lens) <= 1:
+            rows = torch.tensor([r for r, n in enumerate(new_lens) if n], dtype=torch.int64,
+                                pin_memory=True).to(lens.device, non_blocking=True)
+            gaining = self.block_table[rows], lens[rows]
+        self.step = Step(new_lens, self.lengths, slots, cu, lens, gaining)
         self.lens, self.free_count = lens, left
         self.lengths, self.free = after, self.free - need
         return self.step
@@ -108,15 +115,11 @@ class PagedCache:
     def decode(self, layer: int, q, k, v, scale=None) -> torch.Tensor:
         """One token of each request that gains one: keep its key and value, and attend to all
         that the request holds."""
-        new_lens = self._open().new_lens
-        if max(new_lens) > 1:
+        step = self._open()
+        if max(step.new_lens) > 1:
             raise RuntimeError("decode() is for steps of one token a request")
         self.append(layer, k, v)
-        table, lens = self.block_table, self.step.seq_lens
-        if min(new_lens) == 0:
-            rows = torch.tensor([r for r, n in enumerate(new_lens) if n], pin_memory=True).to(
-                lens.device, non_blocking=True)
-            table, lens = table[rows], lens[rows]
+        table, lens = step.gaining or (self.block_table, step.seq_lens)
         return ops.cache_attention(q, self.k_cache[layer], self.v_cache[layer], self.k_scale[layer],
                                    self.v_scale[layer], table, lens, scale)
 
