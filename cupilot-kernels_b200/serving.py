@@ -8,6 +8,8 @@ for each request, and the stack of free blocks.  A step is
         out = cache.prefill(layer, q, k, v)   # whole prompts (requests that held nothing), or
         out = cache.decode(layer, q, k, v)    # one token for each request that gains one
 
+A step is one or the other: `prefill` and `decode` refuse what is not theirs, and
+`cancel` takes back a step that was begun and is not to be.
 `begin` works out the step's lengths on the host (the caller knows them) and
 everything else on the GPU; nothing synchronises.  The keys and values of a
 prompt are attended to in 16 bits as they come and kept in 8 bits for the
@@ -34,7 +36,8 @@ class Step:
     cu_seqlens: torch.Tensor       # new tokens before each request
     seq_lens: torch.Tensor         # tokens after the step
     # Where some requests gain one token and the others none: the former's table rows and lengths.
-    gaining: Optional[Tuple[torch.Tensor, torch.Tensor]] = None
+    gaining: Optional[Tuple[torch.Tensor, torch.Tensor]]
+    before: Tuple[torch.Tensor, torch.Tensor, int]   # lengths, free blocks (device, host) before the step
 
 
 class PagedCache:
@@ -94,10 +97,20 @@ class PagedCache:
             rows = torch.tensor([r for r, n in enumerate(new_lens) if n], dtype=torch.int64,
                                 pin_memory=True).to(lens.device, non_blocking=True)
             gaining = self.block_table[rows], lens[rows]
-        self.step = Step(new_lens, self.lengths, slots, cu, lens, gaining)
+        self.step = Step(new_lens, self.lengths, slots, cu, lens, gaining,
+                         (self.lens, self.free_count, self.free))
         self.lens, self.free_count = lens, left
         self.lengths, self.free = after, self.free - need
         return self.step
+
+    def cancel(self) -> None:
+        """Take back the step that `begin` opened: the requests hold what they held before it, and its
+        blocks are free.  (Codes that it wrote count for nothing; the scale of a block that was partly
+        filled stays as its tokens may have raised it.)"""
+        step = self._open()
+        self.lens, self.free_count, self.free = step.before
+        self.lengths = step.contexts
+        self.step = None
 
     def append(self, layer: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Keep the step's keys and values (tokens, kv_heads, dim)."""
@@ -108,7 +121,7 @@ class PagedCache:
         """The step's prompts: keep their keys and values, and attend to them."""
         step = self._open()
         if any(n and c for n, c in zip(step.new_lens, step.contexts)):
-            raise RuntimeError("prefill() is for requests that held no token")
+            raise RuntimeError("prefill() is for requests that held no token (cancel() takes the step back)")
         self.append(layer, k, v)
         return ops.prompt_attention(q, k, v, self.step.cu_seqlens, scale=scale)
 
@@ -117,7 +130,7 @@ class PagedCache:
         that the request holds."""
         step = self._open()
         if max(step.new_lens) > 1:
-            raise RuntimeError("decode() is for steps of one token a request")
+            raise RuntimeError("decode() is for steps of one token a request (cancel() takes the step back)")
         self.append(layer, k, v)
         table, lens = step.gaining or (self.block_table, step.seq_lens)
         return ops.cache_attention(q, self.k_cache[layer], self.v_cache[layer], self.k_scale[layer],

@@ -50,3 +50,49 @@ def test_the_requests_that_gain_a_token_are_the_ones_attended_for(serving, ops):
         want = ops.cache_attention(q, c.k_cache[layer], c.v_cache[layer], c.k_scale[layer], c.v_scale[layer],
                                    c.block_table[rows], step.seq_lens[rows])
         assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("codes", ["int8", "e4m3"])
+def test_a_step_that_is_taken_back_leaves_no_token(serving, codes):
+    """A step that prefill() and decode() refuse, or that is not wanted any more: the cache goes on as
+    if it had not been begun."""
+    caches = [_cache(serving, codes=codes) for _ in range(2)]
+    outs = []
+    for c, mixed in zip(caches, (False, True)):
+        c.begin([17, 0, 30])
+        c.prefill(0, *_qkv(47))
+        if mixed:
+            before = (c.lengths, c.free, c.lens.tolist(), c.free_count.item())
+            c.begin([1, 20, 1])                       # a prompt among running requests
+            with pytest.raises(RuntimeError, match="one token a request"):
+                c.decode(0, *_qkv(22, seed=3))
+            with pytest.raises(RuntimeError, match="held no token"):
+                c.prefill(0, *_qkv(22, seed=3))
+            c.cancel()
+            assert (c.lengths, c.free, c.lens.tolist(), c.free_count.item()) == before
+            with pytest.raises(RuntimeError, match="begin"):
+                c.decode(0, *_qkv(2))
+        c.begin([1, 0, 1])
+        outs.append(c.decode(0, *_qkv(2, seed=4)))
+        c.begin([0, 20, 0])
+        outs.append(c.prefill(0, *_qkv(20, seed=5)))
+        c.begin([1, 1, 1])
+        outs.append(c.decode(0, *_qkv(3, seed=6)))
+        c.release(2)
+        assert sorted(c.free_blocks[:c.free].tolist() + c.block_table[0, :2].tolist()
+                      + c.block_table[1, :2].tolist()) == list(range(8))
+    assert all(torch.equal(a, b) for a, b in zip(outs[:3], outs[3:]))
+
+
+def test_cancel_wants_a_step(serving):
+    c = _cache(serving)
+    for _ in range(2):
+        with pytest.raises(RuntimeError, match="begin"):
+            c.cancel()
+        c.begin([1, 0, 0])
+        c.cancel()
+    c.begin([16, 0, 0])
+    c.release(0)
+    with pytest.raises(RuntimeError, match="begin"):
+        c.cancel()
+    assert c.free == 8 and c.free_count.item() == 8
