@@ -877,7 +877,7 @@ int check(const b2g_cache_attention_desc* d) {
   if (!d || d->requests < 0 || d->heads < 0 || d->kv_heads < 0 || d->dim <= 0 ||
       d->num_blocks < 0 || d->table_width < 0 || d->table_ld < d->table_width ||
       (d->dtype != B2G_F16 && d->dtype != B2G_BF16) ||
-      (d->codes != B2G_I8 && d->codes != B2G_E4M3) || !(d->scale >= 0.f))
+      (d->codes != B2G_I8 && d->codes != B2G_E4M3) || !(d->scale >= 0.f && std::isfinite(d->scale)))
     return B2G_ERR_INVALID_ARG;
   if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return B2G_ERR_INVALID_ARG;
   if (d->block_size < 16 || d->block_size > 256 || (d->block_size & (d->block_size - 1)) ||

@@ -841,7 +841,7 @@ extern "C" int b2g_prompt_attention(const b2g_prompt_attention_desc* d, b2g_stre
   using namespace b2g::prompt;
   if (!d || d->tokens < 0 || d->tokens_k < 0 || d->sequences < 0 || d->heads < 0 ||
       d->kv_heads < 0 || d->dim <= 0 || (d->dtype != B2G_F16 && d->dtype != B2G_BF16) ||
-      !(d->scale >= 0.f))
+      !(d->scale >= 0.f && std::isfinite(d->scale)))
     return B2G_ERR_INVALID_ARG;
   if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return B2G_ERR_INVALID_ARG;
   if (d->tokens == 0 || d->heads == 0) return B2G_OK;

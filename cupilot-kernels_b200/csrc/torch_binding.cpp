@@ -14,6 +14,7 @@
 #include <torch/extension.h>
 
 #include <atomic>
+#include <cmath>
 
 #include "../../include/b2g_gemm.h"
 #include "../../include/b2g_serving.h"
@@ -634,10 +635,12 @@ void cache_append(const at::Tensor& k, const at::Tensor& v, const at::Tensor& sl
   check_status(b2g_cache_append(&d, stream.stream()), "b2g_cache_append");
 }
 
+// (0 selects the default in the C ABI: a scale that fp32 rounds to 0 must not become that)
 float scale_of(c10::optional<double> scale) {
   if (!scale.has_value()) return 0.f;
-  TORCH_CHECK(*scale > 0, "scale must be positive");
-  return static_cast<float>(*scale);
+  const float s = static_cast<float>(*scale);
+  TORCH_CHECK(s > 0 && std::isfinite(s), "scale must be positive and finite in 32 bits, got ", *scale);
+  return s;
 }
 
 // The output, with its log sums where asked for.

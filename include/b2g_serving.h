@@ -93,7 +93,8 @@ B2G_API int b2g_cache_append(const b2g_cache_append_desc* desc, b2g_stream_t str
  * Lengths are cut to table_width * block_size; a block number outside the
  * cache leaves its tokens out.  num_blocks * kv_heads * block_size, the rows
  * that the kernel counts, stays below 2^31 (so does table_width * block_size).  A request without tokens gives zeros, and
- * -infinity for its log sum.  scale 0 selects 1/sqrt(dim).
+ * -infinity for its log sum.  scale 0 selects 1/sqrt(dim), below 0 or not
+ * finite is an error.
  * q: (requests, heads, dim), element (r, j, i) at r * q_row_stride +
  * j * q_head_stride + i (multiples of 8, 16-byte aligned); out: dense
  * (requests, heads, dim); lse: null, or (requests, heads) fp32 natural
@@ -131,8 +132,8 @@ B2G_API int b2g_cache_attention(const b2g_cache_attention_desc* desc, b2g_stream
  * q, k, v, out: element (t, h, i) at t * token_stride + h * head_stride + i,
  * strides multiples of 8 elements, 16-byte aligned; heads a multiple of
  * kv_heads, heads / kv_heads <= 128; dim a multiple of 16, at most 128.
- * scale 0 selects 1/sqrt(dim), below 0 is an error.  lse: null, or (tokens,
- * heads) fp32.
+ * scale 0 selects 1/sqrt(dim), below 0 or not finite is an error.  lse: null,
+ * or (tokens, heads) fp32.
  */
 typedef struct b2g_prompt_attention_desc {
   int32_t dtype;                /* b2g_dtype of q, k, v and out            */

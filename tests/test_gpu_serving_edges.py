@@ -94,3 +94,14 @@ def test_tables_of_4086_requests_first_in_a_process():
     code = f"import sys\nsys.path.insert(0, {str(REPO)!r})" + _ONE_TOKEN_EACH.format(n=4086)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+# -------------------------------------------------------------- refused scales
+@pytest.mark.parametrize("scale", [1e-60, 1e60, math.inf, math.nan, 0.0])
+def test_scales_that_32_bits_do_not_hold_are_refused(ops, scale):
+    q = torch.randn(4, 2, 64, device="cuda").half()
+    with pytest.raises(RuntimeError, match="scale must be positive"):
+        ops.prompt_attention(q, q, q, _dev([0, 4]), scale=scale)
+    kc, ks = torch.zeros(2, 2, 16, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, device="cuda")
+    with pytest.raises(RuntimeError, match="scale must be positive"):
+        ops.cache_attention(q, kc, kc, ks, ks, _dev([[0]] * 4), _dev([1] * 4), scale)
