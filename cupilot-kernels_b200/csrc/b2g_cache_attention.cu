@@ -642,8 +642,10 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
         }
         // The scales, which may still be on their way, complete the stage.
         if (lane >= first && lane < first + L::kPieces)
-          // A block outside the cache leaves its tokens out.
-          scales[slot * L::kPieces + lane - first] = make_float2(id >= 0 ? ks : __uint_as_float(kNoBlock), vs);
+          // A block outside the cache leaves its tokens out.  (kNoBlock is one of the NaN: a scale that
+          // is NaN goes on as another one.)
+          scales[slot * L::kPieces + lane - first] =
+              make_float2(id >= 0 ? (ks == ks ? ks : NAN) : __uint_as_float(kNoBlock), vs);
         __syncwarp();
         if (lane == 0) ptx::mbar_arrive(&full[slot]);
         __syncwarp();

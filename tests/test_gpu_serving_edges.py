@@ -105,3 +105,17 @@ def test_scales_that_32_bits_do_not_hold_are_refused(ops, scale):
     kc, ks = torch.zeros(2, 2, 16, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, device="cuda")
     with pytest.raises(RuntimeError, match="scale must be positive"):
         ops.cache_attention(q, kc, kc, ks, ks, _dev([[0]] * 4), _dev([1] * 4), scale)
+
+
+# --------------------------------------------------- key scales that are NaN
+@pytest.mark.parametrize("bits", [0xffffffff, 0x7fffffff, 0x7fc00000])
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_key_scale_of_nan_is_not_a_missing_block(ops, d, bits):
+    g = torch.Generator().manual_seed(d)
+    kc, ks = _random_cache(g, 4, 1, 16, d, torch.int8)
+    ks[2].view(torch.int32)[:] = bits - (1 << 32) if bits >> 31 else bits
+    q = torch.randn(2, 2, d, generator=g).half().cuda()
+    args = [x.cuda() for x in (kc, kc, ks, torch.ones_like(ks))]
+    out, lse = ops.cache_attention(q, *args, _dev([[0, 1], [2, 3]]), _dev([30, 30]), return_lse=True)
+    assert torch.isfinite(out[0]).all() and torch.isfinite(lse[0]).all()
+    assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
