@@ -11,6 +11,9 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/extension.h>
 
 #include <atomic>
@@ -643,6 +646,24 @@ float scale_of(c10::optional<double> scale) {
   return s;
 }
 
+// Where an input wants a gradient the results say that they have one, and the
+// backward pass that comes to them raises: there is none.
+void no_backward(const char* name, std::initializer_list<at::Tensor> inputs,
+                 std::initializer_list<at::Tensor> results) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor& x : inputs) {
+    if (!x.requires_grad()) continue;
+    torch::autograd::edge_list edges;
+    for (const at::Tensor& y : inputs) edges.push_back(torch::autograd::impl::gradient_edge(y));
+    auto node = std::shared_ptr<torch::autograd::Error>(
+        new torch::autograd::Error(std::string(name) + " has no backward pass", std::move(edges)),
+        torch::autograd::deleteNode);
+    for (at::Tensor r : results)
+      if (r.defined()) torch::autograd::set_history(r, node);
+    return;
+  }
+}
+
 // The output, with its log sums where asked for.
 py::object with_lse(const at::Tensor& out, const at::Tensor& lse, bool both) {
   if (both) return py::cast(std::make_pair(out, lse));
@@ -705,6 +726,7 @@ py::object cache_attention(const at::Tensor& q, const at::Tensor& k_cache, const
   d.workspace_bytes = ws;
   auto stream = at::cuda::getCurrentCUDAStream(q.device().index());
   check_status(b2g_cache_attention(&d, stream.stream()), "b2g_cache_attention");
+  no_backward("cache_attention", {q, k_scale, v_scale}, {out, lse});
   return with_lse(out, lse, return_lse);
 }
 
@@ -768,6 +790,7 @@ py::object prompt_attention(const at::Tensor& q, const at::Tensor& k, const at::
   d.lse = return_lse ? lse.data_ptr<float>() : nullptr;
   auto stream = at::cuda::getCurrentCUDAStream(q.device().index());
   check_status(b2g_prompt_attention(&d, stream.stream()), "b2g_prompt_attention");
+  no_backward("prompt_attention", {q, k, v}, {out, lse});
   return with_lse(out, lse, return_lse);
 }
 

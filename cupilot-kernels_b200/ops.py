@@ -148,7 +148,8 @@ batched_matmul_out = _ext.batched_matmul_out
 # The operators of a paged 8-bit key/value cache (`serving.PagedCache` runs
 # them together).  All of them work on the current stream and neither
 # synchronise nor read a device value on the host; lengths, tables and slots
-# are int32 / int64 CUDA tensors.
+# are int32 / int64 CUDA tensors.  There is no backward pass: one that comes to
+# an attention's result raises, and what the cache keeps is a constant.
 
 
 def block_tables(context_lens, new_lens, block_table, free_blocks, free_count, total_tokens,

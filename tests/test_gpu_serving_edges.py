@@ -119,3 +119,30 @@ def test_a_key_scale_of_nan_is_not_a_missing_block(ops, d, bits):
     out, lse = ops.cache_attention(q, *args, _dev([[0, 1], [2, 3]]), _dev([30, 30]), return_lse=True)
     assert torch.isfinite(out[0]).all() and torch.isfinite(lse[0]).all()
     assert torch.isnan(out[1]).all() and torch.isnan(lse[1]).all()
+
+
+# ---------------------------------------------------------------- gradients
+def test_a_backward_pass_that_is_not_there_raises(ops):
+    """Forward results are the same where an input wants a gradient, which is not lost silently."""
+    q, k = (torch.randn(4, h, 64, device="cuda").half() for h in (4, 2))
+    kc, ks = torch.zeros(2, 2, 16, 64, dtype=torch.int8, device="cuda"), torch.zeros(2, 2, device="cuda")
+    cu, table, lens = _dev([0, 4]), _dev([[0]] * 4), _dev([1] * 4)
+    calls = [lambda q, k, lse: ops.prompt_attention(q, k, k, cu, return_lse=lse),
+             lambda q, k, lse: ops.cache_attention(q, kc, kc, ks, ks, table, lens, return_lse=lse)]
+    for f in calls:
+        want = f(q, k, True)
+        assert not want[0].requires_grad
+        leaf, other = q.clone().requires_grad_(), k.clone().requires_grad_()
+        for part in (0, 1):
+            got = f(leaf, other, True)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+            with pytest.raises(RuntimeError, match="no backward pass"):
+                got[part].sum().backward()
+        with pytest.raises(RuntimeError, match="no backward pass"):
+            (f(leaf * 2, other, False).sum() + leaf.sum()).backward()
+        assert leaf.grad is None
+        for context in (torch.no_grad, torch.inference_mode):
+            with context():
+                assert not f(leaf, other, False).requires_grad
+    with pytest.raises(RuntimeError, match="no backward pass"):
+        ops.prompt_attention(q, other, k, cu).sum().backward()
