@@ -883,10 +883,19 @@ int check(const b2g_cache_attention_desc* d) {
     return B2G_ERR_INVALID_ARG;
   if (d->heads > 0 && (d->kv_heads == 0 || d->heads % d->kv_heads)) return B2G_ERR_INVALID_ARG;
   if (d->block_size < 16 || d->block_size > 256 || (d->block_size & (d->block_size - 1)) ||
-      d->dim % 16 || d->dim > 128 || d->num_blocks > 0x7fffffff ||
-      d->table_width * d->block_size > 0x7fffff00 || d->requests > (1 << 20) ||
-      d->num_blocks * d->kv_heads * d->block_size > 0x7fffffff || d->heads > (1 << 16) || d->requests * d->heads > 0x7fffffff)
+      d->dim % 16 || d->dim > 128)
     return B2G_ERR_UNSUPPORTED;
+  // (each factor before the products that it stands in)
+  if (d->num_blocks > 0x7fffffff || d->heads > (1 << 16) || d->kv_heads > (1 << 16) ||
+      d->requests > (1 << 20) || d->table_width > 0x7fffffff ||
+      d->table_width * d->block_size > 0x7fffff00 ||
+      d->num_blocks * d->kv_heads * d->block_size > 0x7fffffff || d->requests * d->heads > 0x7fffffff)
+    return B2G_ERR_UNSUPPORTED;
+  // The kernel counts the tiles of all requests in 32 bits: requests that share blocks, or wrong
+  // lengths, may fill whole rows of a wide table.
+  const int rows = d->kv_heads > 0 && d->heads / d->kv_heads > 8 ? 16 : 8;
+  const int64_t tiles = cdiv(d->table_width * d->block_size, tile_tokens(d->dim <= 64 ? 64 : 128, rows));
+  if (d->requests * tiles > 0x7fffffff) return B2G_ERR_UNSUPPORTED;
   return B2G_OK;
 }
 

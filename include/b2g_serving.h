@@ -92,8 +92,9 @@ B2G_API int b2g_cache_append(const b2g_cache_append_desc* desc, b2g_stream_t str
  *   n < seq_lens[r], token n in block block_table[r][n / block_size]
  * Lengths are cut to table_width * block_size; a block number outside the
  * cache leaves its tokens out.  num_blocks * kv_heads * block_size, the rows
- * that the kernel counts, stays below 2^31 (so does table_width * block_size).  A request without tokens gives zeros, and
- * -infinity for its log sum.  scale 0 selects 1/sqrt(dim), below 0 or not
+ * that the kernel counts, stays below 2^31; so do table_width * block_size and
+ * requests * table_width * block_size / 64.  A request without tokens gives
+ * zeros, and -infinity for its log sum.  scale 0 selects 1/sqrt(dim), below 0 or not
  * finite is an error.
  * q: (requests, heads, dim), element (r, j, i) at r * q_row_stride +
  * j * q_head_stride + i (multiples of 8, 16-byte aligned); out: dense
