@@ -96,6 +96,20 @@ def test_tables_of_4086_requests_first_in_a_process():
     assert r.returncode == 0, r.stderr[-2000:]
 
 
+def test_tables_of_lengths_that_sum_past_31_bits(ops):
+    """Out of the documented range: wrong slots at most, and no entry from beyond the stack."""
+    most = (1 << 31) - 1
+    free = torch.arange(100, 108, dtype=torch.int32, device="cuda")
+    big = torch.full((4, 9), -7, dtype=torch.int32, device="cuda")
+    slots, cu, lens, left = ops.block_tables(_dev([0, 5, 0, 40]), _dev([most] * 4), big[:, :6], free, _dev([8]),
+                                             64, 16)
+    assert (big[:, 6:] == -7).all()
+    entries = big[:, :6]
+    assert ((entries == -7) | (entries == -1) | ((entries >= 100) & (entries < 108))).all()
+    assert slots.shape == (64,) and ((slots >= -1) & (slots < 108 * 16)).all()
+    _no_error(ops)
+
+
 # -------------------------------------------------------------- refused scales
 @pytest.mark.parametrize("scale", [1e-60, 1e60, math.inf, math.nan, 0.0])
 def test_scales_that_32_bits_do_not_hold_are_refused(ops, scale):
@@ -146,3 +160,50 @@ def test_a_backward_pass_that_is_not_there_raises(ops):
                 assert not f(leaf, other, False).requires_grad
     with pytest.raises(RuntimeError, match="no backward pass"):
         ops.prompt_attention(q, other, k, cu).sum().backward()
+
+
+# ------------------------------------------------------------------- C ABI
+def test_the_c_entries_give_what_the_torch_entries_give(ops, capi):
+    g = torch.Generator(device="cuda").manual_seed(40)
+    h, group, d, bs, n = 2, 4, 80, 32, 70
+    stream = torch.cuda.current_stream().cuda_stream
+    ctx, new = _dev([5, 0]), _dev([30, 40])
+    free, count = torch.arange(6, dtype=torch.int32, device="cuda"), _dev([6])
+    tables = [_dev([[7, -1, -1], [-1, -1, -1]]) for _ in range(2)]
+    want = ops.block_tables(ctx, new, tables[0], free, count, n, bs)
+    got = [torch.empty_like(x) for x in want]
+    assert capi.block_tables(ctx.data_ptr(), new.data_ptr(), 2, tables[1].data_ptr(), 3, 3, free.data_ptr(), 6,
+                             count.data_ptr(), n, bs, *(x.data_ptr() for x in got), stream=stream) == capi.B2G_OK
+    assert torch.equal(*tables) and all(torch.equal(a, b) for a, b in zip(got, want))
+
+    q = torch.randn(n, h * group, d, generator=g, device="cuda").bfloat16()
+    k, v = (torch.randn(n, h, d, generator=g, device="cuda").bfloat16() for _ in range(2))
+    caches = [[torch.zeros(8, h, bs, d, dtype=torch.int8, device="cuda") for _ in range(2)]
+              + [torch.zeros(8, h, device="cuda") for _ in range(2)] for _ in range(2)]
+    slots, cu, lens, _ = want
+    ops.cache_append(k, v, slots, *caches[0])
+    desc = capi.CacheAppendDesc(capi.BF16, capi.I8, n, h, d, 8, bs, k.data_ptr(), h * d, d, v.data_ptr(), h * d, d,
+                                slots.data_ptr(), *(x.data_ptr() for x in caches[1]))
+    assert capi.cache_append(desc, stream) == capi.B2G_OK
+    assert all(torch.equal(a, b) for a, b in zip(*caches))
+
+    out, lse = ops.cache_attention(q[:2], *caches[0], tables[0], lens, return_lse=True)
+    mine, mine_lse = torch.empty_like(out), torch.empty_like(lse)
+    kc, vc, ks, vs = caches[0]
+    desc = capi.CacheAttentionDesc(capi.BF16, capi.I8, 2, h * group, h, d, 8, bs, q.data_ptr(), h * group * d, d,
+                                   kc.data_ptr(), vc.data_ptr(), ks.data_ptr(), vs.data_ptr(), tables[0].data_ptr(),
+                                   3, 3, lens.data_ptr(), 0.0, mine.data_ptr(), mine_lse.data_ptr(), None, 0)
+    assert capi.cache_attention(desc, stream) == capi.B2G_ERR_WORKSPACE
+    space = torch.empty(capi.cache_attention_workspace_bytes(desc), dtype=torch.uint8, device="cuda")
+    desc.workspace, desc.workspace_bytes = space.data_ptr(), space.numel()
+    assert capi.cache_attention(desc, stream) == capi.B2G_OK
+    assert torch.equal(mine, out) and torch.equal(mine_lse, lse)
+
+    out, lse = ops.prompt_attention(q, k, v, cu, return_lse=True)
+    mine, mine_lse = torch.empty_like(out), torch.empty_like(lse)
+    desc = capi.PromptAttentionDesc(capi.BF16, 1, n, n, 2, h * group, h, d, q.data_ptr(), h * group * d, d,
+                                    k.data_ptr(), h * d, d, v.data_ptr(), h * d, d, mine.data_ptr(), h * group * d, d,
+                                    cu.data_ptr(), None, 0.0, mine_lse.data_ptr())
+    assert capi.prompt_attention(desc, stream) == capi.B2G_OK
+    assert torch.equal(mine, out) and torch.equal(mine_lse, lse)
+    _no_error(ops)
