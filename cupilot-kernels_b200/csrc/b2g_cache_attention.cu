@@ -8,8 +8,8 @@
 // exactly: a warp's m16n8k16 products take 16 tokens' codes, widened in
 // registers, as the 16 rows and up to 8 (or 2 x 8) of the query heads that
 // share the kv head as the columns, S^T = K Q^T and O^T = V^T P^T, so that a
-// group of 8 heads fills a product.  q is brought to [-1, 1] by a power of two
-// (exact in fp16, where a row's small values may go subnormal), the weights
+// group of 8 heads fills a product.  q is brought to [-2^15, 2^15] by a power of
+// two (exact in fp16 down to 2^-28 of a row's largest value), the weights
 // times their value scales are fp16 of at most 2^15, the largest of a head
 // near 2^7 (11 bits down to 2^-21 of it), sums, maxima and the output are fp32.
 //
@@ -423,9 +423,10 @@ __device__ __forceinline__ void take_query(State<DP, ROWS>& s, const uint4 (&raw
     }
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
     most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
-    const int e = min(max(static_cast<int>(__float_as_uint(most) >> 23) - 126, -126), 126);
+    // The largest comes to [2^14, 2^15): the row's others have fp16's whole range below it.
+    const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 141, -127);
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const float rf = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+    const float rf = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(135 + e) << 23) * 0x1p-8f;
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {

@@ -10,7 +10,8 @@ import pytest
 import torch
 
 from conftest import REPO
-from test_gpu_serving import CODES, DTYPES, _attend, _close, _codes_of, _dev, _ids, _no_error, _random_cache
+from test_gpu_serving import (CODES, DTYPES, LSE_TOL, _attend, _close, _codes_of, _dev, _ids, _no_error,
+                              _random_cache)
 
 pytestmark = pytest.mark.gpu
 
@@ -207,3 +208,41 @@ def test_the_c_entries_give_what_the_torch_entries_give(ops, capi):
     assert capi.prompt_attention(desc, stream) == capi.B2G_OK
     assert torch.equal(mine, out) and torch.equal(mine_lse, lse)
     _no_error(ops)
+
+
+# ------------------------------------------------ cache attention: queries
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_values_beside_a_large_one_in_a_query_keep_their_bits(ops, d, dtype):
+    # values 2^-22 of the row's largest, which the keys do not see
+    codes = torch.float8_e4m3fn
+    g = torch.Generator().manual_seed(d)
+    n, blocks = 200, 13
+    kc, ks = _random_cache(g, blocks, 2, 16, d, codes)
+    vc, vs = _random_cache(g, blocks, 2, 16, d, codes)
+    kc = torch.where(torch.arange(d) == 3, 0, kc.view(torch.uint8)).view(codes)
+    ks = ks * 2.0 ** 13
+    q = (torch.randn(1, 8, d, generator=g) * 2.0 ** -12).to(dtype)
+    q[:, :, 3] = 2.0 ** 10
+    k, v = ((c.double() * s.double()[:, :, None, None]).transpose(1, 2).reshape(-1, 2, d)[:n]
+            for c, s in ((kc, ks), (vc, vs)))
+    want, want_lse = _attend(q.double(), k, v, d ** -0.5)
+    out, lse = ops.cache_attention(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), _dev([list(range(blocks))]),
+                                   _dev([n]), None, True)
+    _close(out, want, dtype)
+    assert (lse.cpu().double() - want_lse).abs().max() <= LSE_TOL
+
+
+@pytest.mark.parametrize("codes", CODES, ids=_ids)
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+def test_queries_of_any_size_give_the_same_scores(ops, dtype, codes):
+    """Powers of two move between the query and the scale: from the type's least normal value to its largest."""
+    g = torch.Generator().manual_seed(50)
+    kc, ks = _random_cache(g, 7, 2, 16, 64, codes)
+    q = torch.randn(1, 8, 64, generator=g).clamp(-3.9, 3.9).to(dtype)
+    q = torch.where(q.abs() < 0.25, 0.25, q)
+    args = [x.cuda() for x in (kc, kc, ks, ks)] + [_dev([list(range(7))]), _dev([100])]
+    want, want_lse = ops.cache_attention(q.cuda(), *args, 0.125, True)
+    for power in (-12, 13) if dtype == torch.float16 else (-115, -60, 60, 110):
+        out, lse = ops.cache_attention(q.cuda() * 2.0 ** power, *args, 0.125 * 2.0 ** -power, True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
