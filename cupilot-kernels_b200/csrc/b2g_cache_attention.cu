@@ -161,11 +161,17 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// 1152 + c for an int8 code c, as the fp16 with bits 0x6400 | (c + 128) is 1024 + (c + 128).
-constexpr float kI8Offset = 1152.f;
+// An int8 code c, with its sign bit turned c + 128, in the low byte of an fp16
+// is the subnormal number (c + 128) 2^-24: what the sum of the products has to
+// lose again is 128 times the query's own sum.  (With an offset of 1152, as
+// normal numbers have it, the log sums of queries with a common part of 10 were
+// off by 1.3e-3, with this one by 2.5e-5; without one, for 32 subtractions a
+// piece, 64 requests of 24000 tokens take 521 us for 504.)  The 2^24 comes back in two parts, with the query's power of
+// two and with the key scale, neither of which then leaves fp32's range.
+constexpr float kI8Offset = 128.f * 0x1p-24f, kI8Query = 0x1p15f, kI8Scale = 0x1p9f;
 
-// Four codes to two fp16 pairs.  OFFSET: int8 codes come as 1152 + c (and the
-// caller takes the 1152 out of the sum).
+// Four codes to two fp16 pairs.  OFFSET: int8 codes come as (128 + c) 2^-24 (and the
+// caller takes the offset out of the sum), else as c.
 template <bool E4M3, bool OFFSET>
 __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
   if (E4M3) {
@@ -175,8 +181,9 @@ __device__ __forceinline__ void widen4(uint32_t w, uint32_t& lo, uint32_t& hi) {
         : "r"(w));
   } else {
     const uint32_t u = w ^ 0x80808080u;
-    lo = __byte_perm(u, 0x64646464u, 0x4140);
-    hi = __byte_perm(u, 0x64646464u, 0x4342);
+    // 0x6400 + u is 1024 + u.
+    lo = __byte_perm(u, OFFSET ? 0u : 0x64646464u, 0x4140);
+    hi = __byte_perm(u, OFFSET ? 0u : 0x64646464u, 0x4342);
     if (!OFFSET) {
       const __half2 off = __half2half2(__ushort_as_half(0x6480));   // 1152
       const __half2 hx = __hsub2(*reinterpret_cast<__half2*>(&lo), off);
@@ -193,7 +200,7 @@ struct State {
   static constexpr int N = ROWS / 8;   // columns of 8 query heads
   uint32_t q[N][DP / 16][2];           // head 8 n + g, the lane's dims
   // Of heads 8 n + 2 c, 8 n + 2 c + 1:
-  float rf[N][2];                      // scale * log2(e) * the power of two that q was divided by
+  float rf[N][2];                      // scale * log2(e) * the powers of two that q and the codes were divided by
   float start[N][2];                   // what S starts from: the int8 offset's share
   float m[N][2], l[N][2];              // maximum so far (log2 units), this lane's part of the sum
   float b[N][2];                       // o is in units of 2^b, l in units of 2^m: b is the largest of
@@ -426,7 +433,9 @@ __device__ __forceinline__ void take_query(State<DP, ROWS>& s, const uint4 (&raw
     // The largest comes to [2^14, 2^15): the row's others have fp16's whole range below it.
     const int e = max(static_cast<int>(__float_as_uint(most) >> 23) - 141, -127);
     const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-    const float rf = a.scale_log2 * __uint_as_float(static_cast<uint32_t>(135 + e) << 23) * 0x1p-8f;
+    // (2^(e + 8) and 2^-8: 2^e itself may be subnormal)
+    const float rf =
+        a.scale_log2 * __uint_as_float(static_cast<uint32_t>(135 + e) << 23) * (E4M3 ? 0x1p-8f : 0x1p-8f * kI8Query);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < DP / 16; ++i) {
@@ -617,7 +626,7 @@ __global__ void __launch_bounds__(Smem<DP, ROWS>::kThreads, Smem<DP, ROWS>::kCta
           }
           ks = vs = 0.f;
           if (id >= 0) {
-            ks = __ldg(a.k_scale + static_cast<int64_t>(id) * a.kv_heads + head);
+            ks = __ldg(a.k_scale + static_cast<int64_t>(id) * a.kv_heads + head) * (E4M3 ? 1.f : kI8Scale);
             vs = __ldg(a.v_scale + static_cast<int64_t>(id) * a.kv_heads + head);
           }
         }

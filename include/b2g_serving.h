@@ -99,7 +99,8 @@ B2G_API int b2g_cache_append(const b2g_cache_append_desc* desc, b2g_stream_t str
  * q: (requests, heads, dim), element (r, j, i) at r * q_row_stride +
  * j * q_head_stride + i (multiples of 8, 16-byte aligned); out: dense
  * (requests, heads, dim); lse: null, or (requests, heads) fp32 natural
- * logarithms of the softmax's sums.
+ * logarithms of the softmax's sums.  (Over int8 codes a score is the difference
+ * of two sums in fp32, an error of up to 2^-13 * scale * k_scale * sum |q|.)
  */
 typedef struct b2g_cache_attention_desc {
   int32_t dtype;                /* b2g_dtype of q and out                  */

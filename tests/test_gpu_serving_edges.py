@@ -243,6 +243,27 @@ def test_queries_of_any_size_give_the_same_scores(ops, dtype, codes):
     q = torch.where(q.abs() < 0.25, 0.25, q)
     args = [x.cuda() for x in (kc, kc, ks, ks)] + [_dev([list(range(7))]), _dev([100])]
     want, want_lse = ops.cache_attention(q.cuda(), *args, 0.125, True)
-    for power in (-12, 13) if dtype == torch.float16 else (-115, -60, 60, 110):
+    for power in (-12, 13) if dtype == torch.float16 else (-115, -60, 60, 110, 122):
         out, lse = ops.cache_attention(q.cuda() * 2.0 ** power, *args, 0.125 * 2.0 ** -power, True)
         assert torch.equal(out, want) and torch.equal(lse, want_lse)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=_ids)
+@pytest.mark.parametrize("bias", [3.0, 10.0])
+def test_log_sums_of_queries_with_a_common_part(ops, bias, dtype):
+    """The products add up bias * (code + offset) dim by dim in 32 bits, of which the offset's share is
+    taken out: 8 additions, each cut at 2^-23 of sums up to 128 |q|_1 in units of ks * scale."""
+    g = torch.Generator().manual_seed(51)
+    n, d, blocks = 1000, 128, 63
+    kc, _ = _random_cache(g, blocks, 1, 16, d, torch.int8)
+    vc, vs = _random_cache(g, blocks, 1, 16, d, torch.int8)
+    ks = torch.full((blocks, 1), 0.03)
+    q = (torch.randn(1, 4, d, generator=g) + bias).to(dtype)
+    k, v = ((c.double() * s.double()[:, :, None, None]).transpose(1, 2).reshape(-1, 1, d)[:n]
+            for c, s in ((kc, ks), (vc, vs)))
+    want, want_lse = _attend(q.double(), k, v, d ** -0.5)
+    out, lse = ops.cache_attention(q.cuda(), kc.cuda(), vc.cuda(), ks.cuda(), vs.cuda(), _dev([list(range(blocks))]),
+                                   _dev([n]), None, True)
+    _close(out, want, dtype)
+    cut = 8 * 2.0 ** -23 * 128 * q.double().abs().sum(-1) * 0.03 * d ** -0.5
+    assert ((lse.cpu().double() - want_lse).abs() <= cut + 2e-5).all()
