@@ -10,8 +10,8 @@ import pytest
 import torch
 
 from conftest import REPO
-from test_gpu_serving import (CODES, DTYPES, LSE_TOL, _attend, _close, _codes_of, _dev, _ids, _no_error,
-                              _random_cache)
+from test_gpu_serving import (CODES, DTYPES, LSE_TOL, _attend, _close, _codes_of, _dev, _ids, _no_error, _random_cache,
+                              _step, _step_state)
 
 pytestmark = pytest.mark.gpu
 
@@ -267,3 +267,26 @@ def test_log_sums_of_queries_with_a_common_part(ops, bias, dtype):
     _close(out, want, dtype)
     cut = 8 * 2.0 ** -23 * 128 * q.double().abs().sum(-1) * 0.03 * d ** -0.5
     assert ((lse.cpu().double() - want_lse).abs() <= cut + 2e-5).all()
+
+
+# ------------------------------------------------------------ a captured step
+def test_a_captured_step_replayed_while_lengths_grow(ops):
+    """The lengths and the stack's count come back as new tensors: copied into the captured inputs between
+    replays, they make the same steps as calls do."""
+    eager, state = _step_state(60), _step_state(60)
+    _step(ops, _step_state(61))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = _step(ops, state)
+    for _ in range(20):
+        want = _step(ops, eager)
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+        for s, (_, lens, left, *_) in ((eager, want), (state, got)):
+            s["lens"].copy_(lens)
+            s["count"].copy_(left)
+        for s in (eager, state):
+            s["q"].mul_(-1.25).clamp_(-8, 8)
+            s["k"].mul_(1.125).clamp_(-8, 8)
+    _no_error(ops)
