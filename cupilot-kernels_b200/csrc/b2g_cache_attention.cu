@@ -8,7 +8,8 @@
 // exactly: a warp's m16n8k16 products take 16 tokens' codes, widened in
 // registers, as the 16 rows and up to 8 (or 2 x 8) of the query heads that
 // share the kv head as the columns, S^T = K Q^T and O^T = V^T P^T, so that a
-// group of 8 heads fills a product.  q is brought to [-2^15, 2^15] by a power of
+// group of 8 heads fills a product (a group of more than 16 is taken 16 at a
+// time, and the cache read once for each 16).  q is brought to [-2^15, 2^15] by a power of
 // two (exact in fp16 down to 2^-28 of a row's largest value), the weights
 // times their value scales are fp16 of at most 2^15, the largest of a head
 // near 2^7 (11 bits down to 2^-21 of it), sums, maxima and the output are fp32.
@@ -22,15 +23,16 @@
 // lengths fill the GPU evenly; what a cut divides is joined by a second small
 // kernel.
 //
-// Measured (GB/s of codes, 6547 being the card's copy rate):
+// Measured in a stream of calls (in brackets: on the GPU alone, a graph of 20
+// calls; GB/s of codes, 6547 being the card's copy rate):
 //   64 requests of 14000 to 31000 tokens, 8 kv heads, 32 heads, dim 128, int8:
-//   462 us, 6550 GB/s; 0.53 ms once the power limit lowers the clock
-//   1 request of 150001 tokens, 4 kv heads, 32 heads, e4m3: 38 us, 4070 GB/s
-//   (some 10 us are start, the cuts' partial results and their join)
-//   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 39 us,
-//   3370 GB/s (the consumers' chains of dependent products, not the loads)
-//   1 request of 997 tokens: 8.8 us, two launches and a handful of dependent
-//   loads
+//   501 us, 6040 GB/s (472, 6410; the power limit lowers the clock in longer runs)
+//   1 request of 150001 tokens, 4 kv heads, 32 heads, e4m3: 39.5 us, 3890 GB/s
+//   (37; some 10 us are start, the cuts' partial results and their join)
+//   48 ragged requests up to 6000 tokens, 56 heads on 8, dim 64, e4m3: 42.9 us,
+//   3090 GB/s (41; the consumers' chains of dependent products, not the loads)
+//   1 request of 997 tokens: 10.3 us (9.1), two launches and a handful of
+//   dependent loads
 // K as the first operand instead of q halves the products (8 heads of 16 rows
 // were empty): 822 -> 475 us together with the TMA ring, whose place registers
 // had before.

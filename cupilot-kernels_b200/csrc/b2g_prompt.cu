@@ -28,10 +28,11 @@
 // that a tile's chain softmax - P V - Q K^T, some 1500 + 1024 cycles and four
 // barriers, sets the pace of a step (2700 to 3000 cycles; a third tile has no
 // room in tensor memory).  Measured:
-//   16384 tokens, 16 heads on 4, dim 128, bf16: 0.83 ms, 1320 TFLOP/s, in a
-//   short burst (the card's cuBLAS burst is 1658); 0.96 ms, 1150, once the
-//   power limit holds the clock at 1.6 GHz (cuBLAS then: 1384)
-//   6 prompts of 700 to 2300 tokens, 32 heads on 8: 0.12 ms, 910 TFLOP/s
+//   16384 tokens, 16 heads on 4, dim 128, bf16: 0.97 ms, 1130 TFLOP/s, in a
+//   stream of calls, where the power limit holds the clock at 1.6 GHz (cuBLAS
+//   then: 1384); 0.83 ms, 1320, in a short burst (cuBLAS: 1658)
+//   6 prompts of 700 to 2300 tokens, 32 heads on 8: 0.143 ms, 770 TFLOP/s in a
+//   stream of calls; 0.121 ms, 910, in a short burst
 // Tried and slower: two threads to a row (four softmax warps a scheduler: S
 // read twice or registers spilled, +15 %), a thread for each tile's products
 // (both tiles' softmax then fall on the same cycles, +25 %), branches around

@@ -32,8 +32,9 @@ int log2_of(int64_t x) {
 // was there) or on the stack (one taken now), and the token that opens a new
 // block writes the table entry.  No CTA reads what another writes, so one
 // launch does it all.  Bound by latency: launch, one load of the lengths,
-// one dependent load of the block, one store (8 requests: 2.5 us; 1000
-// requests with 64000 new tokens: 4.9 us).
+// one dependent load of the block, one store (on the GPU, 8 requests:
+// 2.1 us; 1000 requests with 64000 new tokens: 4.5 us; a call takes 6.5 us of
+// the host for either).
 
 constexpr int64_t kSmallStep = 256;   // requests of a step that the smaller CTAs take
 
@@ -163,9 +164,10 @@ __global__ void __launch_bounds__(THREADS) block_tables_kernel(const TableArgs a
 // grew, the new codes.  The group's owner is the only one that touches the
 // block's codes and scale of that head, so nothing is atomic and the result
 // does not depend on the order.  Bound by memory (2 bytes read and 1 written a
-// value) in the long run, by the warps' chain of loads in a call's few waves:
-// 18000 tokens, 8 heads of 128, blocks of 32: 22 us, 3700 GB/s; 64 single
-// tokens: 3.2 us.
+// value) in the long run, by the warps' chain of loads in a call's few waves,
+// and where a group has more rows than a warp holds (16 of 128 dims) its rows are
+// read twice: 18000 tokens, 8 heads of 128, blocks of 32: 23.9 us, 3460 GB/s in a
+// stream of calls (22.4 on the GPU); 64 single tokens: 4.7 us (2.8).
 constexpr int kAppendWarps = 8;
 struct AppendArgs {
   const uint16_t* x[2];          // keys, values

@@ -207,7 +207,8 @@ def prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k=None, causal=True, scale=
     the last query sees the last key).  A query that sees no key gives zeros.
 
     Returns the output in q's dtype, with `return_lse` also the natural
-    logarithms of the softmax sums (tokens, heads), float32.
+    logarithms of the softmax sums (tokens, heads), float32 (to 7.5e-5 for
+    bf16, 2.7e-6 for fp16).
     """
     return _ext.prompt_attention(q, k, v, cu_seqlens, cu_seqlens_k, causal, scale, return_lse)
 

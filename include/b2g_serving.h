@@ -87,7 +87,7 @@ B2G_API int b2g_cache_append(const b2g_cache_append_desc* desc, b2g_stream_t str
 
 /*
  * One query token per request over the cache, query head j reading kv head
- * j / (heads / kv_heads):
+ * j / (heads / kv_heads) (the cache is read once for every 16 of them):
  *   out[r][j] = sum_n softmax_n(scale * q[r][j] . K[r][n]) V[r][n],
  *   n < seq_lens[r], token n in block block_table[r][n / block_size]
  * Lengths are cut to table_width * block_size; a block number outside the
@@ -135,7 +135,9 @@ B2G_API int b2g_cache_attention(const b2g_cache_attention_desc* desc, b2g_stream
  * strides multiples of 8 elements, 16-byte aligned; heads a multiple of
  * kv_heads, heads / kv_heads <= 128; dim a multiple of 16, at most 128.
  * scale 0 selects 1/sqrt(dim), below 0 or not finite is an error.  lse: null,
- * or (tokens, heads) fp32.
+ * or (tokens, heads) fp32, the natural logarithms of the sums; a part of the
+ * exponentials is a polynomial whose relative error, and so the lse's absolute
+ * one, reaches 7.5e-5 for bf16 and 2.7e-6 for fp16.
  */
 typedef struct b2g_prompt_attention_desc {
   int32_t dtype;                /* b2g_dtype of q, k, v and out            */
